@@ -6,9 +6,10 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import hmx
-from .ops import _f32c, _i64c, _need_cuda, workspace
+from .ops import _f32c, _i64c, _launch, _need_cuda, _one_device, _rows, workspace
 
 N_STATE = 16
 DT_RANK = 16
@@ -106,6 +107,75 @@ class _RMSNorm(torch.autograd.Function):
 
 def rmsnorm(x, scale, eps=1e-6):
     return _RMSNorm.apply(x, scale, eps)
+
+
+def _norm_operands(what, x, residual, scale, eps):
+    """Checks the operands of the residual-add norms; -> device, (T, d) views of x and residual, 1 for bfloat16."""
+    device = _one_device(what, x, residual, scale)
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise hmx.HmxError(f"{what}: x is float32 or bfloat16, got {x.dtype}")
+    if x.dim() == 0 or not 1 <= x.shape[-1] <= 32768:
+        raise hmx.HmxError(f"{what}: the last dimension of x holds 1 to 32768 values, got {tuple(x.shape)}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise hmx.HmxError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+    if scale.shape != (x.shape[-1],) or scale.dtype != torch.float32:
+        raise hmx.HmxError(f"{what}: scale is float32 ({x.shape[-1]},), got {scale.dtype} {tuple(scale.shape)}")
+    if not eps >= 0.0:
+        raise hmx.HmxError(f"{what}: eps is {eps}")
+    return device, _rows(x), None if residual is None else _rows(residual), int(x.dtype == torch.bfloat16)
+
+
+class _AddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, scale, eps):
+        device, x2, r2, bf16 = _norm_operands("add_rmsnorm", x, residual, scale, eps)
+        T, d = x2.shape
+        scale = scale.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=device)
+        s = torch.empty(x.shape, dtype=x.dtype, device=device) if r2 is not None else None
+        rstd = torch.empty(T, dtype=torch.float32, device=device) if any(ctx.needs_input_grad) else None
+        _launch("hmx_add_rmsnorm_fwd", device, x2.data_ptr(), x2.stride(0), hmx.ptr(r2), 0 if r2 is None else r2.stride(0),
+                scale.data_ptr(), T, d, eps, bf16, hmx.ptr(s), y.data_ptr(), hmx.ptr(rstd))
+        ctx.set_materialize_grads(False)
+        ctx.bf16, ctx.has_residual = bf16, r2 is not None
+        if rstd is not None:
+            ctx.save_for_backward(s if r2 is not None else x, scale, rstd)
+        return (y, s) if r2 is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, scale, rstd = ctx.saved_tensors
+        if dy is None:                            # nothing arrives at y: the sum passes its own gradient on
+            return ds, (ds if ctx.has_residual else None), None, None
+        device, d = s.device, s.shape[-1]
+        s2, dy2 = _rows(s).contiguous(), dy.reshape(-1, d).contiguous()
+        ds2 = None if ds is None else ds.reshape(-1, d).contiguous()
+        T = s2.shape[0]
+        dx = torch.empty(s.shape, dtype=s.dtype, device=device)
+        dscale = None
+        part = None
+        if ctx.needs_input_grad[2]:
+            if T:
+                part = torch.empty(_L().hmx_add_rmsnorm_bwd_blocks(T, d), d, dtype=torch.float32, device=device)
+            else:
+                dscale = torch.zeros(d, dtype=torch.float32, device=device)
+        _launch("hmx_add_rmsnorm_bwd", device, s2.data_ptr(), scale.data_ptr(), rstd.data_ptr(), dy2.data_ptr(), hmx.ptr(ds2), T,
+                d, ctx.bf16, dx.data_ptr(), hmx.ptr(part))
+        if part is not None:
+            with torch.cuda.device(device):
+                dscale = colsum(part)
+        return dx, (dx if ctx.has_residual else None), dscale, None
+
+
+def add_rmsnorm(x, residual, scale, eps=1e-6):
+    """s = x + residual (rounded to their type), y = s * (mean(s^2) + eps)^(-1/2) * scale -> (y, s).
+
+    x and residual (..., d) are float32 or bfloat16 with any strides, 1 <= d <= 32768, scale (d,) is float32; sums are
+    float32.  residual None: the norm of x, -> (y, x).  Gradients flow from y and from s to x, residual and scale."""
+    if residual is None:
+        return _AddRMSNorm.apply(x, None, scale, eps), x
+    return _AddRMSNorm.apply(x, residual, scale, eps)
 
 
 # ------------------------------------------------------------------------------- deferred weight gradients

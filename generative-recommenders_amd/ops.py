@@ -30,6 +30,31 @@ def _i64c(t):
     return t.contiguous()
 
 
+def _one_device(what, *tensors):
+    """The GPU that every tensor given (None: left out) lies on; raises when one lies elsewhere."""
+    _need_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise hmx.HmxError(f"{what}: the tensors lie on different devices ({', '.join(sorted(map(str, devices)))})")
+    return devices.pop()
+
+
+def _launch(name, device, *args):
+    """Calls an entry point on `device` and its current stream, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        code = getattr(hmx.lib(), name)(*args, hmx.current_stream())
+    else:
+        with torch.cuda.device(device):
+            code = getattr(hmx.lib(), name)(*args, hmx.current_stream())
+    hmx.check(code, name)
+
+
+def _rows(t):
+    """(..., d) as a (rows, d) view whose columns are contiguous (a copy only where the strides allow no such view)."""
+    t2 = t.reshape(-1, t.shape[-1])
+    return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
+
+
 def _validate_ids(ids, n_rows, what):
     """Opt-in host check reproducing nn.Embedding's IndexError (costs a device sync)."""
     if CHECK_IDS and ids.numel():

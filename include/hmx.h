@@ -644,6 +644,47 @@ int hmx_attn_fwd(const float* q, const float* kv, const float* drop, int64_t B, 
 int hmx_attn_bwd(const float* q, const float* kv, const float* drop, const float* p, const float* dout, int64_t B,
                  int64_t Lq, int64_t Lk, int64_t d, int64_t H, float* dq, float* dkv, float* ds, float* wv, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * The answer path: residual add + RMS norm of a model's states, tables in 4 bits, items drawn from scores.
+ * ------------------------------------------------------------------------------- */
+
+/* s = x + residual (rounded to the tensors' type), y = s * (mean(s^2) + eps)^(-1/2) * scale over the last dimension.
+ * x, residual, s, y are fp32 (bf16 = 0) or bfloat16 (bf16 = 1), scale and rstd fp32; sums in fp32.  x and residual are
+ * (T, d) with row strides ldx / ldr in elements (0: one row for all), s, y contiguous.  residual NULL: the norm of x
+ * (s may then be NULL).  rstd (T) or NULL receives the factor for the backward pass.  1 <= d <= 32768, eps >= 0. */
+int hmx_add_rmsnorm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* scale, int64_t T,
+                        int64_t d, float eps, int bf16, void* s, void* y, float* rstd, void* stream);
+
+/* Its gradient: dx (T, d), the gradient of x and of residual alike, from dy and ds (NULL: no gradient arrives at s), all
+ * contiguous; dscale_part (hmx_add_rmsnorm_bwd_blocks(T, d), d) or NULL receives partial rows whose column sums
+ * (hmx_colsum_f32) are the gradient of scale. */
+int64_t hmx_add_rmsnorm_bwd_blocks(int64_t T, int64_t d);
+int hmx_add_rmsnorm_bwd(const void* s, const float* scale, const float* rstd, const void* dy, const void* ds, int64_t T,
+                        int64_t d, int bf16, void* dx, float* dscale_part, void* stream);
+
+/* Block-scaled formats: 32 consecutive values of a row share one scale byte b that stands for 2^(b - 127); "mx8" holds a
+ * value as e4m3 (a byte), "mx4" as e2m1 (half a byte: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign; the value with the even
+ * index in the low half).  A row of d values takes dp = 32 ceil(d / 32) codes, the ones past d zero.  A block's scale is
+ * the least power of two 2^e, -126 <= e <= 127, with amax <= limit * 2^e (limit 448 or 6; 2^0 for a block of zeros), so
+ * no value is cut off; values are rounded to nearest even.  A block that holds a NaN or an infinity gets scale byte 255
+ * and zero codes, and stands for NaN.  Codes and scales are contiguous, codes 16-byte aligned.
+ *
+ * hmx_add_rmsnorm_mx8: hmx_add_rmsnorm_fwd with y in mx8 (from the unrounded fp32 y): codes (T, dp), scales (T, dp / 32). */
+int hmx_add_rmsnorm_mx8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* scale, int64_t T,
+                        int64_t d, float eps, int bf16, void* s, void* codes, void* scales, void* stream);
+
+/* A (n, d) table (fp32, or bfloat16 where bf16 = 1; row stride ld in elements) in mx4: codes (n, dp / 2), scales
+ * (n, dp / 32), and the values that mx4 (bits = 4) or mx8 (bits = 8) codes stand for, (n, d) fp32 or bfloat16: exact in
+ * both, infinite from 2^128 on. */
+int hmx_mx4_quantize(const void* table, int64_t ld, int64_t n, int64_t d, int bf16, void* codes, void* scales, void* stream);
+int hmx_mx_dequantize(const void* codes, const void* scales, int64_t n, int64_t d, int bits, int bf16, void* out, void* stream);
+
+/* out (M, N) = x (M, K) * W^T for an mx4 table W (N, K).  x_kind 0: fp32 rows of stride ldx (elements), all 24 bits of a
+ * value take part; 1: bfloat16; 2: mx8 codes (ldx = dp) with x_scales (M, dp / 32).  Sums in fp32; out contiguous, fp32 or
+ * bfloat16 (out_bf16 = 1). */
+int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, int x_kind, int64_t M, const void* codes, const void* scales,
+                   int64_t N, int64_t K, int out_bf16, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

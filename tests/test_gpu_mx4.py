@@ -1,0 +1,266 @@
+"""mx_ops.quantize_mx4 / dequantize_mx4 / linear_mx4 against plain forms in 64 bits.
+
+Quantisation is exact arithmetic up to its one rounding: codes and scales are compared for equality.  linear_mx4 multiplies
+exact operands and adds K products in fp32 in some order: off by at most (K + 16) u of the sum of their magnitudes (the 16:
+the terms that an fp32 x is cut into, the joins of waves), u = 2^-24; a bfloat16 result adds eps / 2 = 2^-8 of the value."""
+import pytest
+import torch
+
+from generative_recommenders_amd import hmx, mx_ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+GRID = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+
+
+def plain_quantize(w):
+    """Exponents (128: not finite) and values of the definition, in 64 bits on the CPU, nearest code by search."""
+    w = w.double().cpu()
+    n, d = w.shape
+    p = torch.zeros(n, mx_ops.padded(d), dtype=torch.float64)
+    p[:, :d] = w
+    p = p.view(n, -1, 32)
+    amax = p.abs().amax(2)
+    finite = torch.isfinite(p).all(2)
+    e = torch.full(amax.shape, -126.0, dtype=torch.float64)
+    for k in range(-126, 127):
+        e = torch.where(amax > 6 * 2.0 ** k, torch.full_like(e, k + 1), e)
+    e = torch.where(amax == 0, torch.zeros_like(e), e)
+    e = torch.where(finite, e, torch.full_like(e, 128.0))
+    unit = torch.exp2(torch.where(finite, e, torch.zeros_like(e))).unsqueeze(2)
+    a = torch.where(finite.unsqueeze(2), p / unit, torch.zeros_like(p))
+    dist = (a.abs().unsqueeze(3) - GRID).abs()
+    dist[..., 1::2] *= 1 + 1e-12                         # a tie goes to the even code
+    code = dist.argmin(3)
+    values = torch.copysign(GRID[code], a) * unit
+    values = torch.where(finite.unsqueeze(2), values, torch.full_like(values, float("nan")))
+    return e, code + 8 * torch.signbit(a), values.view(n, -1)
+
+
+def unpack(codes):
+    return torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
+
+
+def table(n, d, dtype=torch.float32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, d, generator=g) * torch.logspace(-2, 1, n).unsqueeze(1)).to(dtype)
+
+
+def check_quantize(w):
+    codes, scales = mx_ops.quantize_mx4(w)
+    n, d = w.shape
+    e, code, values = plain_quantize(w)
+    assert torch.equal(scales.cpu(), (e + 127).to(torch.uint8))
+    assert torch.equal(unpack(codes.cpu()).view(code.shape), code.to(torch.uint8))
+    for dt in (torch.float32, torch.bfloat16):
+        got = mx_ops.dequantize_mx4(codes, scales, d, dt).cpu()
+        want = values[:, :d].to(dt)         # exact but for 4 * 2^126 = 2^128, next to the largest fp32: infinity in either type
+        same = (got == want) | (got.isnan() & want.isnan())
+        assert got.shape == (n, d) and bool(same.all()), (int((~same).sum()), dt)
+    return codes, scales
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 31), (5, 32), (7, 33), (1000, 60), (513, 64), (65, 100), (9, 1000), (2, 5001)])
+def test_quantize(n, d, dtype):
+    check_quantize(table(n, d, dtype).to(DEV))
+
+
+def test_quantize_ties_borders_and_special_values():
+    w = torch.zeros(12, 64)
+    w[0, :16] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0, -0.0])
+    w[1, 0] = 6.0
+    w[2, 0] = torch.nextafter(torch.tensor(6.0), torch.tensor(7.0))
+    w[3, 40] = float("nan")
+    w[4, 3] = float("-inf")
+    w[5] = torch.finfo(torch.float32).max
+    w[6] = torch.finfo(torch.float32).min
+    w[7] = 1e-45
+    w[8] = 2.0 ** -126
+    w[9, :32] = torch.linspace(-6, 6, 32)
+    w[10, ::2] = 3e-39
+    codes, scales = check_quantize(w.to(DEV))
+    assert int(scales[3, 0]) == 127 and int(scales[3, 1]) == 255 and int(scales[11, 0]) == 127
+
+
+def test_quantize_strides_and_shapes():
+    w = table(60, 64, seed=2).to(DEV)
+    want = check_quantize(w)
+    wide = torch.zeros(60, 131, device=DEV)
+    wide[:, 1:65] = w
+    for v in (wide[:, 1:65], w.t().contiguous().t(), w.view(3, 20, 64)):
+        codes, scales = mx_ops.quantize_mx4(v)
+        assert torch.equal(codes.view(60, 32), want[0]) and torch.equal(scales.view(60, 2), want[1])
+    codes, scales = mx_ops.quantize_mx4(w[:1].expand(5, 64))
+    assert torch.equal(codes, want[0][:1].expand(5, 32))
+    codes, scales = mx_ops.quantize_mx4(torch.empty(0, 40, device=DEV))
+    assert codes.shape == (0, 32) and scales.shape == (0, 2)
+    assert mx_ops.dequantize_mx4(codes, scales, 40).shape == (0, 40)
+
+
+def operands(m, n, k, kind, seed=0):
+    """-> x as the call takes it, its scales, x and W in 64 bits, codes, scales."""
+    codes, scales = mx_ops.quantize_mx4(table(n, k, seed=seed).to(DEV))
+    w = mx_ops.dequantize_mx4(codes, scales, k, torch.float32).double()
+    g = torch.Generator().manual_seed(seed + 1)
+    x = torch.randn(m, k, generator=g).to(DEV)
+    if kind == "mx8":
+        ones = torch.ones(k, device=DEV)
+        q, s, _ = mx_ops.add_rmsnorm_mx8(x, None, ones)
+        return q, s, mx_ops.dequantize_mx8(q, s, k, torch.float32).double(), w, codes, scales
+    x = x.to(torch.float32 if kind == "f32" else torch.bfloat16)
+    return x, None, x.double(), w, codes, scales
+
+
+def check_linear(out, x64, w64, out_dtype=torch.float32):
+    want, mag = x64 @ w64.t(), x64.abs() @ w64.abs().t()
+    tol = (x64.shape[1] + 16) * U * mag + 1e-37
+    if out_dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * (want.abs() + tol)
+    assert out.dtype == out_dtype and out.shape == want.shape
+    err = (out.double() - want).abs()
+    assert not bool((~(err <= tol)).any()), float((err / tol).nan_to_num(1e9).max())
+
+
+KS = [1, 31, 32, 33, 60, 64, 65, 96, 100, 127, 128, 129, 200, 256, 260, 515, 1000, 2048, 4133]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mx8"])
+@pytest.mark.parametrize("k", KS)
+def test_linear_widths(k, kind):
+    for m, n in ((1, 1), (1, 77), (3, 64), (4, 130), (5, 17), (16, 200), (17, 63), (33, 65)):
+        x, xs, x64, w64, codes, scales = operands(m, n, k, kind, seed=k)
+        check_linear(mx_ops.linear_mx4(x, codes, scales, xs), x64, w64)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mx8"])
+@pytest.mark.parametrize("m,n,k", [(1, 5003, 64), (2, 20001, 60), (16, 9001, 32), (64, 3001, 64), (7, 4097, 128), (100, 515, 96),
+                                   (1, 2053, 1024), (32, 1031, 4096), (65, 300, 777), (1, 40, 8192)])
+def test_linear_sizes(m, n, k, kind):
+    x, xs, x64, w64, codes, scales = operands(m, n, k, kind, seed=3)
+    check_linear(mx_ops.linear_mx4(x, codes, scales, xs), x64, w64)
+    check_linear(mx_ops.linear_mx4(x, codes, scales, xs, out_dtype=torch.bfloat16), x64, w64, torch.bfloat16)
+
+
+def test_linear_keeps_all_bits_of_float32():
+    """x that differs in its last bits only: a product with fewer of them would give zero."""
+    codes, scales = mx_ops.quantize_mx4(torch.tensor([[1.0, -1.0]], device=DEV).repeat(70, 1))
+    for base in (1.0, 1e-20, 1e30):
+        a = torch.tensor(base)
+        b = torch.nextafter(a, torch.tensor(float("inf")))
+        out = mx_ops.linear_mx4(torch.stack([b, a]).to(DEV).unsqueeze(0), codes, scales)
+        assert bool((out.cpu() == (b - a)).all())
+
+
+@pytest.mark.parametrize("k", [32, 64, 128, 300])
+@pytest.mark.parametrize("m", [1, 3, 9, 20])
+def test_linear_not_finite(m, k):
+    w = table(200, k, seed=5).to(DEV)
+    w[37, k // 2] = float("nan")
+    w[150, 0] = float("inf")
+    codes, scales = mx_ops.quantize_mx4(w)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(1)).to(DEV)
+    for xx in (x, x.bfloat16()):
+        out = mx_ops.linear_mx4(xx, codes, scales)
+        assert bool(out[:, [37, 150]].isnan().all())
+        keep = torch.ones(200, dtype=torch.bool, device=DEV)
+        keep[[37, 150]] = False
+        w64 = mx_ops.dequantize_mx4(codes, scales, k, torch.float32).double()
+        check_linear(out[:, keep], xx.double(), w64[keep])
+        bad = xx.clone()
+        bad[m - 1, 0] = float("inf")
+        out = mx_ops.linear_mx4(bad, codes, scales)
+        assert not bool(torch.isfinite(out[m - 1]).any())
+        check_linear(out[:m - 1, keep], xx[:m - 1].double(), w64[keep])
+    nonzero = mx_ops.dequantize_mx4(codes, scales, k, torch.float32)[:, 0] != 0
+    keep &= nonzero
+    big = torch.zeros(m, k, device=DEV)
+    big[:, 0] = float("-inf")
+    out = mx_ops.linear_mx4(big, codes, scales)
+    assert bool((out[:, keep] == -float("inf") * torch.sign(w64[keep, 0]).float()).all())
+    big[:, 0] = torch.finfo(torch.float32).max
+    tiny = mx_ops.quantize_mx4(w * 2.0 ** -20)
+    check_linear(mx_ops.linear_mx4(big, *tiny)[:, keep], big.double(), mx_ops.dequantize_mx4(*tiny, k, torch.float32).double()[keep])
+
+
+def test_linear_every_scale_byte():
+    """One row for each scale byte: values from 2^-127 to 6 2^127 times an x that keeps the product in range."""
+    codes = torch.full((256, 16), 0x27, dtype=torch.uint8, device=DEV)           # 6, 1, 6, 1, ...
+    scales = torch.arange(256, dtype=torch.uint8, device=DEV).view(256, 1)
+    e = torch.arange(256, dtype=torch.float64) - 127
+    want = 16 * 7 * torch.exp2(e)
+    for x0 in (2.0 ** -10, 1.0, 2.0 ** 10):
+        for m, kind in ((1, torch.float32), (1, torch.bfloat16), (6, torch.float32)):
+            out = mx_ops.linear_mx4(torch.full((m, 32), x0, dtype=kind, device=DEV), codes, scales).cpu().double()
+            w = (want * x0).float().double()
+            ok = (w >= 2.0 ** -116) & (w < 2.0 ** 128) & (e < 125)   # smaller products meet the denormal range of the sum
+            assert torch.equal(out[:, ok], w[ok].expand(m, -1)) and bool(out[:, 255].isnan().all())
+
+
+def test_linear_strides_shapes_and_empty():
+    x, _, x64, w64, codes, scales = operands(12, 90, 200, "f32", seed=8)
+    want = mx_ops.linear_mx4(x, codes, scales)
+    check_linear(want, x64, w64)
+    wide = torch.full((12, 333), float("nan"), device=DEV)
+    wide[:, 7:207] = x
+    assert torch.equal(mx_ops.linear_mx4(wide[:, 7:207], codes, scales), want)
+    assert torch.equal(mx_ops.linear_mx4(x.t().contiguous().t(), codes, scales), want)
+    assert torch.equal(mx_ops.linear_mx4(x.view(3, 4, 200), codes, scales).view(12, 90), want)
+    assert torch.equal(mx_ops.linear_mx4(x[0], codes, scales), mx_ops.linear_mx4(x[:1], codes, scales)[0])
+    assert torch.equal(mx_ops.linear_mx4(x[:1].expand(12, 200), codes, scales)[11], want[0])
+    assert torch.equal(mx_ops.linear_mx4(x, codes[10:30], scales[10:30]), want[:, 10:30])
+    off = torch.zeros(codes.numel() + 1, dtype=torch.uint8, device=DEV)[1:].view_as(codes).copy_(codes)
+    assert torch.equal(mx_ops.linear_mx4(x, off, scales), want)
+    assert mx_ops.linear_mx4(x[:0], codes, scales).shape == (0, 90)
+    assert mx_ops.linear_mx4(x, codes[:0], scales[:0]).shape == (12, 0)
+
+
+def test_linear_offsets_past_32_bits():
+    n, m = (1 << 26) + 3, 33                             # 2.2e9 outputs
+    g = torch.Generator(device=DEV).manual_seed(4)
+    codes = torch.randint(0, 256, (n, 16), dtype=torch.uint8, device=DEV, generator=g)
+    scales = torch.randint(125, 129, (n, 1), dtype=torch.uint8, device=DEV, generator=g)
+    x = torch.randn(m, 32, device=DEV, generator=g).bfloat16()
+    out = mx_ops.linear_mx4(x, codes, scales)
+    for lo in (0, n // 2, n - 1000):
+        w = mx_ops.dequantize_mx4(codes[lo:lo + 1000], scales[lo:lo + 1000], None, torch.float32).double()
+        check_linear(out[:, lo:lo + 1000], x.double(), w)
+
+
+def test_refusals():
+    x, _, _, _, codes, scales = operands(4, 50, 64, "f32")
+    q, s, _ = mx_ops.add_rmsnorm_mx8(x, None, torch.ones(64, device=DEV))
+    calls = [lambda: mx_ops.quantize_mx4(x.half()), lambda: mx_ops.quantize_mx4(x.cpu()),
+             lambda: mx_ops.quantize_mx4(torch.zeros(4, 0, device=DEV)),
+             lambda: mx_ops.dequantize_mx4(codes, scales[:3]), lambda: mx_ops.dequantize_mx4(codes, scales, 32),
+             lambda: mx_ops.dequantize_mx4(codes, scales, 65), lambda: mx_ops.dequantize_mx4(codes, scales, 64, torch.float16),
+             lambda: mx_ops.dequantize_mx8(codes, scales), lambda: mx_ops.dequantize_mx4(codes.int(), scales),
+             lambda: mx_ops.linear_mx4(x[:, :32], codes, scales), lambda: mx_ops.linear_mx4(x.half(), codes, scales),
+             lambda: mx_ops.linear_mx4(x, codes, scales, s), lambda: mx_ops.linear_mx4(q, codes, scales),
+             lambda: mx_ops.linear_mx4(q, codes, scales, s[:2]), lambda: mx_ops.linear_mx4(x.cpu(), codes, scales),
+             lambda: mx_ops.linear_mx4(x, codes, scales.cpu()), lambda: mx_ops.linear_mx4(x, codes, scales, out_dtype=torch.half),
+             lambda: mx_ops.linear_mx4(x, codes.view(5, 10, 32), scales.view(5, 10, 2))]
+    for call in calls:
+        with pytest.raises(hmx.HmxError):
+            call()
+
+
+def test_graph_and_stream():
+    x, _, x64, w64, codes, scales = operands(3, 3001, 64, "bf16", seed=6)
+    xl, _, _, _, cl, sl = operands(3, 301, 1000, "f32", seed=7)
+    graph = torch.cuda.CUDAGraph()
+    xs = x.clone()
+    with torch.cuda.graph(graph):
+        out, long = mx_ops.linear_mx4(xs, codes, scales), mx_ops.linear_mx4(xl, cl, sl)
+    for k in (1.0, -2.0, 0.5):
+        xs.copy_(k * x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, mx_ops.linear_mx4(xs, codes, scales)) and torch.equal(long, mx_ops.linear_mx4(xl, cl, sl))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = mx_ops.linear_mx4(xs, codes, scales)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(again, out)
