@@ -563,3 +563,52 @@ def topk_merge(cand_ids, cand_scores):
     hmx.check(hmx.lib().hmx_topk_merge(hmx.ptr(ci), hmx.ptr(cs), S, nq, k, hmx.ptr(ids), hmx.ptr(sc),
                                        hmx.current_stream()), "hmx_topk_merge")
     return ids, sc
+
+
+# --------------------------------------------------------------------------- sampling from scores
+def _row_setting(what, name, value, dtype, n_rows, device):
+    """A setting of sample_logits: a number for every row, or a (n_rows,) tensor -> (tensor or None, number)."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.dtype != dtype or value.shape != (n_rows,):
+        raise hmx.HmxError(f"{what}: {name} is a number or a {dtype} tensor ({n_rows},), got {value.dtype} {tuple(value.shape)}")
+    if value.device != device:
+        raise hmx.HmxError(f"{what}: {name} lies on {value.device}, logits on {device}")
+    return value.contiguous(), 0
+
+
+@torch.no_grad()
+def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Draws items from rows of scores -> (ids int64, probs float32), both of u's shape.
+
+    logits (..., V) float32 or bfloat16; u (...) or (..., draws) in [0, 1), float32 or float64: the random numbers, one for
+    each draw (draws of a row are independent, with replacement).  w_i = exp((l_i - max l) / temperature); kept are the
+    top_k highest (ties: lowest index first; 0: all), of these the fewest that hold top_p of their mass, highest first
+    (1: all), of these the ones with w_i >= min_p (0: all).  The draw is the first kept i in index order whose running sum
+    of w exceeds u times the kept mass; probs is its share of that mass.  Every setting is a number or one per row
+    ((rows,) float32; top_k int32).  temperature 0 takes the highest score.  -infinity and NaN are never drawn; a row that
+    holds nothing else gives id -1 and probability 0.  Same inputs, same results: sums do not depend on their order."""
+    device = _one_device("sample_logits", logits, u)
+    if logits.dtype not in (torch.float32, torch.bfloat16) or logits.dim() < 1 or logits.shape[-1] < 1:
+        raise hmx.HmxError(f"sample_logits: logits are float32 or bfloat16 rows, got {logits.dtype} {tuple(logits.shape)}")
+    lead = logits.shape[:-1]
+    if u.dtype not in (torch.float32, torch.float64) or u.shape[:len(lead)] != lead or u.dim() > len(lead) + 1:
+        raise hmx.HmxError(f"sample_logits: u is float32 or float64 of shape {tuple(lead)} or {tuple(lead)} and a number of draws, "
+                           f"got {u.dtype} {tuple(u.shape)}")
+    rows = _rows(logits)
+    b, v = rows.shape
+    t, t_all = _row_setting("sample_logits", "temperature", temperature, torch.float32, b, device)
+    k, k_all = _row_setting("sample_logits", "top_k", top_k, torch.int32, b, device)
+    p, p_all = _row_setting("sample_logits", "top_p", top_p, torch.float32, b, device)
+    mp, mp_all = _row_setting("sample_logits", "min_p", min_p, torch.float32, b, device)
+    if not 0.0 <= t_all < float("inf") or k_all < 0 or not 0.0 <= p_all <= 1.0 or not 0.0 <= mp_all <= 1.0:
+        raise hmx.HmxError(f"sample_logits: temperature {t_all}, top_k {k_all}, top_p {p_all}, min_p {mp_all}: a finite "
+                           "temperature >= 0, top_k >= 0, top_p and min_p in [0, 1] are wanted")
+    draws = u.shape[-1] if u.dim() > len(lead) else 1
+    u = u.contiguous()
+    ids = torch.empty(u.shape, dtype=torch.int64, device=device)
+    probs = torch.empty(u.shape, dtype=torch.float32, device=device)
+    _launch("hmx_sample_logits", device, rows.data_ptr(), rows.stride(0), b, v, int(logits.dtype == torch.bfloat16), u.data_ptr(),
+            int(u.dtype == torch.float64), draws, hmx.ptr(t), hmx.ptr(k), hmx.ptr(p), hmx.ptr(mp), float(t_all), int(k_all),
+            float(p_all), float(mp_all), ids.data_ptr(), probs.data_ptr())
+    return ids, probs

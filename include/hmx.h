@@ -685,6 +685,24 @@ int hmx_mx_dequantize(const void* codes, const void* scales, int64_t n, int64_t 
 int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, int x_kind, int64_t M, const void* codes, const void* scales,
                    int64_t N, int64_t K, int out_bf16, void* out, void* stream);
 
+/* Draws from rows of scores.  For row b of logits (B, V) (fp32, or bfloat16 where bf16 = 1; row stride ld in elements):
+ *   w_i = exp((l_i - max l) / temperature); candidates are all but -infinity and NaN;
+ *   kept are the top_k candidates first by (l descending, i ascending) (top_k <= 0: all); of these, in that order, the
+ *   shortest prefix that holds at least top_p of their mass (top_p >= 1: all; <= 0: the first); of these the ones with
+ *   w_i >= min_p (<= 0: all, > 1: as 1);
+ *   ids[b, s] = the first kept i in index order whose running sum of w exceeds u[b, s] * (mass of the kept), and
+ *   probs[b, s] = w_i / (mass of the kept).
+ * A temperature that is not positive and finite means the first candidate by (l descending, i ascending), probability 1.
+ * Infinite maxima share the mass alone.  A row without candidates gives id -1 and probability 0.
+ * u (B, draws) in [0, 1), fp64 where u_f64 = 1, else fp32; NaN and negative numbers count as 0, 1 and above as just
+ * below 1.  temperature, top_k, top_p, min_p (B) or NULL: then the numbers behind them hold for every row.  Sums are
+ * integers of a fixed unit per row (at most 2^-51 of the largest weight where the row's mass is below 2^11), so results
+ * do not depend on the order of any addition.  V < 2^31, B < 2^22. */
+int hmx_sample_logits(const void* logits, int64_t ld, int64_t B, int64_t V, int bf16, const void* u, int u_f64, int64_t draws,
+                      const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                      double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all, int64_t* ids, float* probs,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

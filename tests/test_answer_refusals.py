@@ -52,3 +52,14 @@ def test_python_entries_refuse_cpu_tensors():
                  lambda: mx_ops.linear_mx4(x, torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8))):
         with pytest.raises(hmx.HmxError):
             call()
+
+
+def test_sample_entry():
+    L = hmx.lib()
+    good = dict(logits=P, ld=64, B=4, V=64, bf16=0, u=P, u64=0, draws=1, t=None, k=None, p=None, mp=None, ta=1.0, ka=0, pa=1.0,
+                mpa=0.0, ids=P, probs=P, stream=None)
+    for bad in (dict(logits=None), dict(ld=-1), dict(B=-1), dict(V=0), dict(V=1 << 31), dict(u=None), dict(draws=-1),
+                dict(ids=None), dict(probs=None), dict(B=1 << 22)):
+        assert L.hmx_sample_logits(*{**good, **bad}.values()) == EINVAL, bad
+    assert L.hmx_sample_logits(*{**good, "B": 0, "logits": None}.values()) == 0
+    assert L.hmx_sample_logits(*{**good, "draws": 0}.values()) == 0
