@@ -4,18 +4,24 @@
 // that order whose mass is at least top_p of theirs; of these the ones with w_i >= min_p.  A draw is the first kept i in
 // INDEX order whose running sum of w passes u * (kept mass): no sort of the row is needed, only the border of the kept set.
 //
-// Weights are fp64 (z exactly as far as fp64 goes, exp by table and polynomial, 2e-16) turned into integers w * 2^s, with s
-// the largest scale at which the row's mass fits 62 bits (51 at most): integer sums do not depend on their order, so LDS
-// and global atomics, any split of a row and any number of waves give the same set and the same draw.
+// Weights are fp64 (z exactly as far as fp64 goes, exp by table and polynomial, 1e-15) turned into integers w * 2^s, with s
+// the largest scale at which the row's mass is sure to fit 62 bits (51 at most): integer sums do not depend on their order,
+// so LDS and global atomics, any split of a row and any number of waves give the same set and the same draw.
 //
-// How the border is found, with as few looks at the row as its settings allow:
-//   top_k: the k-th largest of the maxima of groups of elements is a value that at least k elements reach; what reaches it
-//     is gathered into a list, and the list does the rest (top_p and min_p on top of top_k included).
-//   top_p: masses of 4096 bins of equal width in l.  What lies so far below the maximum that V of it weigh less than half of
-//     1 - top_p is summed without a bin.  One more look sums the tiles of the row above the border's bin and gathers that
-//     bin's few elements, which are sorted for the border itself; the draw goes by the sums of the tiles.
-//   Where a list overflows (equal scores, scores that differ in their last bits): equal ranges of the ordered 32-bit key,
-//     until a range fits the list or is one key, whose border is the index of its r-th element.
+// What bounds it: at four cycles a wave an instruction per element costs 0.9 us for 33.5 M elements on the whole card, so the
+// few instructions that every element meets come first, the 25 of a weight where they can be spared:
+//   bfloat16: one look counts the 16-bit values (4096 counters for 2^-6 <= |l| < 2^10, a list for the rest), which gives
+//     every border exactly: a value and how many of its elements are kept.
+//   fp32, top_k: the k-th largest of the maxima of groups of elements is a value that at least k elements reach; what
+//     reaches it is gathered into a list, and the list does the rest (top_p and min_p on top of top_k included).
+//   fp32, top_p: masses of 4096 bins of equal width in l.  What lies so far below the maximum that V of it weigh less than
+//     half of 1 - top_p is summed without a bin.
+//   Then one look at the row sums, tile by tile of 1024 elements or more, the weights above the border, counts the elements
+//   at the border value (or gathers the border bin's few), and the draws go by the tiles' running sums.
+//   Where a list overflows (equal scores, scores that differ in their last bits): counts or masses of equal ranges of the
+//   ordered 32-bit key, three looks at most, until a range is one key.
+// One block does a row on its own; few long rows are cut into segments for the looks at all elements, with one block a row
+// between them.
 #include "hmx_common.h"
 
 #include <algorithm>
@@ -23,16 +29,17 @@
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kBins = 4096;                // four per thread
+constexpr int kBins = 4096;                // bins, tiles and list entries: four per thread
 constexpr int kPer = kBins / kThreads;
-constexpr int kList = 4096;
+constexpr int kTile = 1024;                // elements of a tile at least: one step of a wave
 constexpr int kSmall = 2048;               // rows up to this length go into the list whole
-constexpr int kTiles = 4096;               // tiles of a row at most (their running sums stay in LDS), four per thread
+constexpr int kMaxSplit = 64;              // blocks a row is cut over at most (64 groups of each have their maximum)
 constexpr uint32_t kLowestKey = 0x00800000u;        // the key after that of -infinity
+constexpr float kMaxFloat = 3.402823466e38f;
 constexpr float kRange = 32.f;             // bins reach down to exp(-32) of the largest weight
+constexpr uint32_t kFirstMag = (127 - 6) << 7;      // bfloat16 magnitudes with a counter: 2^-6 up to 2^10
 
 typedef unsigned long long u64;
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct SampleArgs {
@@ -47,7 +54,7 @@ struct SampleArgs {
     int64_t k;
     int64_t* ids;
     float* probs;
-    uint32_t tile;                                   // elements of a tile, a multiple of 256
+    uint32_t tile;                                   // elements of a tile, a multiple of kTile
 };
 
 // ------------------------------------------------------------------------------- elements
@@ -60,68 +67,79 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 __device__ __forceinline__ bool candidate(float l) { return l > -__builtin_inff(); }      // neither -infinity nor NaN
 
-// Elements i .. i + 3 of a row (NaN past its end).  Rows start anywhere: the loads need only the type's own alignment.
+// Four consecutive elements as they lie in memory (rows start anywhere: the loads need only the type's own alignment), and
+// their values.  Kept apart so that a load can be in flight while earlier elements are used.
 template <typename T>
-__device__ __forceinline__ void load4(const T* row, uint32_t i, uint32_t V, float (&v)[4]) {
-    if (i + 4 <= V) {
-        if constexpr (sizeof(T) == 4) {
-            f32x4 a;
-            __builtin_memcpy(&a, row + i, 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = a[e];
-        } else {
-            bf16x4 a;
-            __builtin_memcpy(&a, row + i, 8);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (float)a[e];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = i < V && i + e < V ? (float)row[i + e] : __builtin_nanf("");
+struct Raw;
+template <>
+struct Raw<float> {
+    f32x4 v;
+    __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(&v, p, 16); }
+    __device__ __forceinline__ float get(int e) const { return v[e]; }
+};
+template <>
+struct Raw<__bf16> {
+    uint2 v;
+    __device__ __forceinline__ void load(const __bf16* p) { __builtin_memcpy(&v, p, 8); }
+    __device__ __forceinline__ float get(int e) const {
+        const uint32_t w = e < 2 ? v.x : v.y;
+        return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
     }
-}
+};
 
-// f(value, index) for the elements of [lo, hi), `threads` threads in steps of four, four steps' loads ahead of their use.
-template <typename T, typename F>
+// f(four values, index of the first) for the elements of [lo, hi), hi >= 4, by `threads` threads (all of them take part in
+// every step; values outside are NaN), DEPTH steps' loads in flight.  The body stays one step of code, the last step its
+// masking apart: most users run it a few times only, and then fetching instructions is what it costs.
+template <int DEPTH, typename T, typename F>
 __device__ __forceinline__ void each_element(const T* row, uint32_t lo, uint32_t hi, int thread, int threads, F f) {
-    constexpr int U = 4;
-    for (uint32_t i0 = lo; i0 < hi; i0 += threads * 4 * U) {
-        float v[U][4];
+    const uint32_t stride = threads * 4, steps = (hi - lo + stride - 1) / stride, last = hi - 4;
+    uint32_t i = lo + thread * 4;
+    Raw<T> ahead[DEPTH];
 #pragma unroll
-        for (int q = 0; q < U; ++q) load4(row, i0 + (q * threads + thread) * 4, hi, v[q]);
+    for (int q = 0; q < DEPTH; ++q) ahead[q].load(row + std::min(i + q * stride, last));
+#pragma unroll 1
+    for (uint32_t n = 0; n < steps; ++n, i += stride) {
+        const Raw<T> v = ahead[0];
 #pragma unroll
-        for (int q = 0; q < U; ++q)
+        for (int q = 0; q + 1 < DEPTH; ++q) ahead[q] = ahead[q + 1];
+        ahead[DEPTH - 1].load(row + std::min(i + DEPTH * stride, last));
+        float l[4] = {v.get(0), v.get(1), v.get(2), v.get(3)};
+        uint32_t first = i;
+        if (n + 1 == steps) {                       // past the end: the row's last four, without what came before
+            first = std::min(i, last);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f(v[q][e], i0 + (q * threads + thread) * 4 + e);
+            for (int e = 0; e < 4; ++e) l[e] = first + e >= i ? l[e] : __builtin_nanf("");
+        }
+        f(l, first);
     }
 }
 
+// ------------------------------------------------------------------------------- weights
 // What a row's weights and bins are computed with.
 struct Row {
-    float lmax, bin_scale;          // bins per unit of l
+    uint32_t top;                   // key of the maximum
+    float lmax_f, bin_scale;        // the maximum (at most the largest finite number), bins per unit of l
+    int scale;                      // units are 2^-scale
+    double lmax;                    // the maximum (1e300 for infinity: all that is finite is nothing beside it)
     double inv_t, step;             // step: 128 / (T ln 2)
     double log_min_p;               // -infinity: off
-    double cut;                     // weights of steps below it round to zero units
-    int scale;                      // units are 2^-scale
+    double cut;                     // steps at which a weight is a quarter of a unit
     double p;                       // 1: off
     int64_t k;                      // 0: off
 };
 
-__device__ __forceinline__ int bin_of(const Row& r, float l) {      // ascending as l falls; kBins: all that lies lower
-    const float t = l == r.lmax ? 0.f : (r.lmax - l) * r.bin_scale;
-    return t < (float)kBins ? (int)t : kBins;
+// Ascending as l falls, kBins: all that lies lower (and -infinity).  NaN: any of them.
+__device__ __forceinline__ int bin_of(const Row& r, float l) {
+    return (int)__builtin_amdgcn_fmed3f((r.lmax_f - l) * r.bin_scale, 0.f, (float)kBins);
 }
-__device__ __forceinline__ double log_weight(const Row& r, float l) {
-    return l == r.lmax ? 0.0 : ((double)l - (double)r.lmax) * r.inv_t;
-}
+__device__ __forceinline__ double log_weight(const Row& r, float l) { return ((double)l - r.lmax) * r.inv_t; }
 
-// exp((l - max) / T) in units of 2^-scale, rounded to an integer (at most 2^51).  With n + x = 128 z / ln 2, |x| <= 1/2 and
-// n = 128 q + i: 2^q * 2^(i / 128) * e^(x ln2 / 128), the last by four terms after 1 (what they leave off: 1e-15), the
-// second from the table.  Adding 1.5 * 2^52 rounds to n and leaves its bits; 2^q goes into the exponent, which stays in
-// range because smaller weights than half a unit end at the cut.
-__device__ __forceinline__ u64 weight(const Row& r, float l, const double* tab) {
-    const double y = l == r.lmax ? 0.0 : ((double)l - (double)r.lmax) * r.step;
-    if (!(y > r.cut)) return 0;
+// exp((l - max) / T) in units of 2^-scale (2^51 at most; 1/4 where it is less), and that rounded to an integer; 0 for
+// -infinity and NaN.  With n + x = 128 z / ln 2, |x| <= 1/2 and n = 128 q + i: 2^q * 2^(i / 128) * e^(x ln2 / 128), the last by
+// four terms after 1 (what they leave off: 1e-15), the second from the table.  Adding 1.5 * 2^52 rounds to n and leaves its
+// bits; 2^q goes into the exponent, which stays in range because of the cut.
+__device__ __forceinline__ double weight_units(const Row& r, float l, const double* tab) {
+    const double y = fmin(fmax(((double)l - r.lmax) * r.step, r.cut), 0.0);      // fmax drops NaN
     const double shifted = y + 6755399441055744.0;
     const int n = (int)(uint32_t)__double_as_longlong(shifted);
     const double x = y - (shifted - 6755399441055744.0);
@@ -130,58 +148,110 @@ __device__ __forceinline__ u64 weight(const Row& r, float l, const double* tab) 
     e = fma(x, e, 0.0054152123481245725);
     e = fma(x, e, 1.0);
     const double m = tab[n & 127] * e;
-    const double w = __longlong_as_double(__double_as_longlong(m) + ((long long)((n >> 7) + r.scale) << 52));
-    return __double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+    return __longlong_as_double(__double_as_longlong(m) + ((long long)((n >> 7) + r.scale) << 52));
+}
+__device__ __forceinline__ u64 weight(const Row& r, float l, const double* tab) {
+    return __double_as_longlong(weight_units(r, l, tab) + 4503599627370496.0) & 0xfffffffffffffull;
+}
+__device__ __forceinline__ bool passes(const Row& r, float l) { return log_weight(r, l) >= r.log_min_p; }
+
+__device__ __forceinline__ u64 share_of(double p, u64 total) {
+    const u64 t = (u64)ceil((p > 0.0 ? p : 0.0) * (double)total);
+    return t < 1 ? 1 : t > total ? total : t;
 }
 
-// The kept set so far: keys above `key`, and of those equal to it the indices up to `idx`.
-struct Border {
-    uint32_t key, idx;
-};
-__device__ __forceinline__ bool inside(const Border& b, uint32_t key, uint32_t i) {
-    return key > b.key || (key == b.key && i <= b.idx);
-}
-__device__ __forceinline__ u64 kept_weight(const Row& r, const Border& in, float l, uint32_t i, const double* tab) {
-    if (!candidate(l) || !inside(in, key_of(l), i)) return 0;
-    return log_weight(r, l) >= r.log_min_p ? weight(r, l, tab) : 0;
+__device__ __forceinline__ Row settings(const SampleArgs& a, int64_t b) {
+    double t = a.temperature ? (double)a.temperature[b] : a.t;
+    const double p = a.top_p ? (double)a.top_p[b] : a.p, mp = a.min_p ? (double)a.min_p[b] : a.mp;
+    Row r;
+    r.k = a.top_k ? a.top_k[b] : a.k;
+    if (!(t > 0.0) || t > 3e38) t = 1.0, r.k = 1;
+    if (r.k < 0 || r.k >= a.V) r.k = 0;
+    r.p = p < 1.0 ? p : 1.0;
+    r.inv_t = 1.0 / t;
+    r.log_min_p = -__builtin_inf();
+    if (mp > 0.0) r.log_min_p = log(mp < 1.0 ? mp : 1.0);
+    r.step = 184.6649652337873 * r.inv_t;                            // 128 / ln 2
+    r.top = 0;
+    r.lmax_f = r.bin_scale = 0.f;
+    r.lmax = r.cut = 0.0;
+    r.scale = 0;
+    return r;
 }
 
-// The largest candidate of a thread's share of [lo, hi) (-infinity: none).
-template <typename T>
-__device__ __forceinline__ float thread_max(const T* row, uint32_t lo, uint32_t hi, int thread, int threads) {
-    float top = -__builtin_inff();
-    each_element(row, lo, hi, thread, threads, [&](float l, uint32_t) { top = fmaxf(top, l); });       // fmaxf drops NaN
-    return top;
+// The maximum, and the scale: the row's mass, at most `most` times the largest weight, has to fit 62 bits.
+__device__ __forceinline__ void set_scale(Row& r, float lmax, float most) {
+    const bool finite = lmax <= kMaxFloat;
+    r.top = key_of(lmax);
+    r.lmax_f = finite ? lmax : kMaxFloat;
+    r.lmax = finite ? (double)lmax : 1e300;
+    const int ex = (int)((__float_as_uint(most) >> 23) & 255) - 126;  // most < 2^ex
+    r.scale = min(51, 62 - ex);
+    r.cut = -128.0 * (double)(r.scale + 2);
 }
+__device__ __forceinline__ void set_bins(Row& r, float range) {
+    r.bin_scale = fminf((float)((double)kBins * r.inv_t) / range, kMaxFloat);
+}
+// For top_p: V elements below the bins' range weigh less than half of what top_p leaves out of a mass of at least `least`.
+__device__ __forceinline__ float range_for(const Row& r, uint32_t V, float least) {
+    const float out = (float)(1.0 - r.p) * least * 0.75f;
+    const float down = 0.6931472f * __builtin_amdgcn_logf(2.f * (float)V / out);
+    return out > 0.f && down < kRange ? fmaxf(down, 0.125f) : kRange;
+}
+// Whether the k-th largest of `groups` maxima leads to a list: groups * ln(groups / (groups - k)) elements reach it where the
+// groups are alike, 1650 of 1024 groups, 2750 of 4096 at most.
+__device__ __forceinline__ bool by_maxima(const Row& r, int groups) { return r.k > 0 && 5 * r.k <= 4 * groups && r.k <= 2000; }
 
 // ------------------------------------------------------------------------------- block sums
-__device__ __forceinline__ u64 shfl_up64(u64 v, int d) {
-    const uint32_t lo = __shfl_up((uint32_t)v, d), hi = __shfl_up((uint32_t)(v >> 32), d);
+// v of the lane that the DPP control names; 0 where there is none, or where the row mask leaves the lane out.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp64(u64 v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, ROWS == 0xf);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, ROWS == 0xf);
     return ((u64)hi << 32) | lo;
 }
-__device__ __forceinline__ u64 wave_incl(u64 v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = shfl_up64(v, d);
-        if (lane >= d) v += o;
-    }
+__device__ __forceinline__ u64 row_incl(u64 v) {                     // inclusive sums in rows of 16 lanes
+    v += dpp64<0x111, 0xf>(v);                                       // shift right by 1, 2, 4, 8 in a row
+    v += dpp64<0x112, 0xf>(v);
+    v += dpp64<0x114, 0xf>(v);
+    v += dpp64<0x118, 0xf>(v);
     return v;
 }
+__device__ __forceinline__ u64 wave_incl(u64 v) {                    // all lanes active
+    v = row_incl(v);
+    v += dpp64<0x142, 0xa>(v);                                       // lane 15 of rows 0 and 2 to rows 1 and 3
+    v += dpp64<0x143, 0xc>(v);                                       // lane 31 to rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {
+    return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+
+// How far a row has come (Mode names what the next look at its elements has to do).
+enum Mode : int { kDone, kGather, kBinning, kTiles, kAlone };
+struct State {
+    Row r;
+    int mode;
+    uint32_t klo, khi;              // gather: from klo on; tiles: weights above khi, klo to khi apart
+    int ties;                       // tiles: 1 = klo == khi and `need` of that key's elements are kept, 0 = the list has them
+    u64 need;                       // elements of the border key, or units of the border bin's mass
+};
 
 struct Shared {
     double tab[128];
     union {
-        u64 mass[kBins];
+        u64 bins[kBins];
         uint32_t count[kBins];
-        u64 run[kList];
-        u64 tile[kTiles];
+        u64 run[kBins];
+        u64 tile[kBins];
     };
     union {
-        u64 list[kList];
-        uint32_t ties[kTiles];
-        float group[kThreads];
+        u64 list[kBins];
+        float group[kBins];
     };
+    uint32_t ties[kBins];
+    State st;
     u64 wsum[kWaves];
     float wmax[kWaves];
     u64 rest, above, target, total, in_bin;
@@ -189,90 +259,53 @@ struct Shared {
 };
 
 __device__ __forceinline__ void make_table(Shared& sh) {
-    if (threadIdx.x < 128) sh.tab[threadIdx.x] = exp2((double)threadIdx.x / 128.0);
+    // 2^(i / 128) from the powers that i's bits stand for: a few roundings, and little code
+    const double root[7] = {1.0054299011128027, 1.0108892860517005, 1.0218971486541166, 1.0442737824274138,
+                            1.0905077326652577, 1.189207115002721, 1.4142135623730951};
+    double v = 1.0;
+#pragma unroll
+    for (int q = 0; q < 7; ++q) v *= (threadIdx.x >> q) & 1 ? root[q] : 1.0;
+    if (threadIdx.x < 128) sh.tab[threadIdx.x] = v;
 }
 
 // Inclusive sums over the block in thread order; *total gets the sum of all.
 __device__ __forceinline__ u64 block_incl(u64 v, Shared& sh, u64* total) {
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     v = wave_incl(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) sh.wsum[wave] = v;
     __syncthreads();
-    u64 before = 0, all = 0;
+    const u64 sums = row_incl(sh.wsum[threadIdx.x & 15]);            // kWaves = 16: one row of lanes
+    *total = lane64(sums, 15);
+    return v + (wave ? lane64(sums, wave - 1) : 0);
+}
+__device__ __forceinline__ float block_max(float v, Shared& sh) {
+    for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wmax[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh.wmax[threadIdx.x & 15];
+    for (int d = 1; d < 16; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+__device__ __forceinline__ float block_sum(float v, Shared& sh) {
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wmax[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh.wmax[threadIdx.x & 15];
+    for (int d = 1; d < 16; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// The place among four values a thread (in thread order) at which their running sum reaches `target` (> 0): sh.bin (kBins
+// where they do not), sh.above before it, sh.in_bin its value.  `extra` comes before the second half of the values.
+__device__ __forceinline__ void find_place(const u64 (&v)[kPer], u64 target, u64 extra, Shared& sh) {
+    u64 all, sum = 0;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        before += i < wave ? sh.wsum[i] : 0;
-        all += sh.wsum[i];
-    }
-    *total = all;
-    return v + before;
-}
-
-// ------------------------------------------------------------------------------- selection
-enum Kind { kCount, kMass };
-
-// Adds one element to the bins; what lies below them goes to the thread's own `rest`.
-template <Kind KIND>
-__device__ __forceinline__ void add_to_bin(const Row& r, float l, int b, u64* mass, uint32_t* count, const double* tab, u64& rest) {
-    if constexpr (KIND == kMass) {
-        const u64 w = weight(r, l, tab);
-        if (b == kBins) rest += w;
-        else atomicAdd(&mass[b], w);
-    } else {
-        if (b == kBins) ++rest;
-        else atomicAdd(&count[b], 1u);
-    }
-}
-
-// Counts or masses of the row's elements inside `in` by bin.  SUB false: bins of bin_of(), the rest apart; true: ranges of
-// 2^shift keys below khi, elements from klo to khi only.
-template <typename T, Kind KIND, bool SUB>
-__device__ __forceinline__ void histogram(const SampleArgs& a, const T* row, const Row& r, const Border& in, uint32_t klo, uint32_t khi,
-                          int shift, Shared& sh) {
-    for (int b = threadIdx.x; b < kBins; b += kThreads) {
-        if (KIND == kMass) sh.mass[b] = 0;
-        else sh.count[b] = 0;
-    }
-    if (threadIdx.x == 0) sh.rest = 0;
-    __syncthreads();
-    u64 rest = 0;
-    each_element(row, 0, a.V, threadIdx.x, kThreads, [&](float l, uint32_t i) {
-        if (!candidate(l)) return;
-        const uint32_t key = key_of(l);
-        if (!inside(in, key, i)) return;
-        if (SUB && (key < klo || key > khi)) return;
-        add_to_bin<KIND>(r, l, SUB ? (int)((khi - key) >> shift) : bin_of(r, l), sh.mass, sh.count, sh.tab, rest);
-    });
-    if (!SUB && rest) atomicAdd(&sh.rest, rest);
-    __syncthreads();
-}
-
-// The first bin at which the running count (mass) reaches `target` (> 0): sh.bin (kBins where the bins do not reach it),
-// sh.above, sh.in_bin, sh.target, and sh.total of all bins and the rest.  share >= 0: the target is that part of the total.
-template <Kind KIND>
-__device__ __forceinline__ void find_bin(u64 target, double share, Shared& sh) {
-    u64 v[kPer], sum = 0;
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        v[q] = KIND == kMass ? sh.mass[kPer * threadIdx.x + q] : (u64)sh.count[kPer * threadIdx.x + q];
-        sum += v[q];
-    }
-    u64 all;
-    u64 upto = block_incl(sum, sh, &all) - sum;
-    const u64 total = all + sh.rest;
-    if (share >= 0.0) {
-        target = (u64)ceil(share * (double)total);
-        target = target < 1 ? 1 : target > total ? total : target;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        sh.bin = kBins;
-        sh.above = all;
-        sh.in_bin = sh.rest;
-        sh.target = target;
-        sh.total = total;
-    }
+    for (int q = 0; q < kPer; ++q) sum += v[q];
+    u64 upto = block_incl(sum, sh, &all) - sum + (threadIdx.x >= kThreads / 2 ? extra : 0);
+    if (threadIdx.x == 0) sh.bin = kBins, sh.above = all + extra, sh.in_bin = 0;
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
@@ -282,172 +315,60 @@ __device__ __forceinline__ void find_bin(u64 target, double share, Shared& sh) {
     __syncthreads();
 }
 
-// The largest key with bin_of >= b (kLowestKey - 1: none); every wave searches for itself, 64 keys at a time.
-__device__ __forceinline__ uint32_t last_key_of_bin(const Row& r, int b) {
-    uint32_t lo = kLowestKey - 1, hi = key_of(r.lmax) + 1;          // holds at lo, not at hi
-    if (b <= 0) return hi - 1;
-    while (hi - lo > 1) {
-        const uint32_t step = (hi - lo - 1) / 64 + 1;
-        const u64 at = (u64)lo + (u64)step * ((threadIdx.x & 63) + 1);
-        const bool yes = at < hi && bin_of(r, value_of((uint32_t)at)) >= b;
-        const int n = __popcll(__ballot(yes));
-        const u64 top = (u64)lo + (u64)step * (n + 1);
-        lo += step * n;
-        hi = top < hi ? (uint32_t)top : hi;
-    }
-    return lo;
-}
-__device__ __forceinline__ uint32_t first_key_of_bin(const Row& r, int b) {      // the smallest key with bin_of <= b
-    return b >= kBins ? kLowestKey : last_key_of_bin(r, b + 1) + 1;
-}
-
+// ------------------------------------------------------------------------------- the list
 __device__ __forceinline__ u64 entry(uint32_t key, uint32_t i) { return ((u64)key << 32) | (uint32_t)~i; }
 __device__ __forceinline__ float entry_value(u64 x) { return value_of((uint32_t)(x >> 32)); }
 
-// Sorts the list's first n entries; DESC: the largest first.  Bitonic: steps of up to 64 stay in a wave's own 128 entries
-// and need no barrier of the block.
+// Sorts n entries that differ; DESC: the largest first.  Up to 256: each goes to the place that the count of those before it
+// names.  More: bitonic; steps of up to 64 stay in a wave's own 128 entries and need no barrier of the block.
 template <bool DESC>
 __device__ __forceinline__ void sort_list(uint32_t n, u64* list) {
-    uint32_t m = 2;
+    __syncthreads();
+    if (n <= 256) {
+        const u64 x = threadIdx.x < n ? list[threadIdx.x] : 0;
+        uint32_t place = 0;
+        if ((threadIdx.x & ~63u) < n)
+            for (uint32_t i = 0; i < n; ++i) place += DESC ? list[i] > x : list[i] < x;
+        __syncthreads();
+        if (threadIdx.x < n) list[place] = x;
+        __syncthreads();
+        return;
+    }
+    uint32_t m = 512;
     while (m < n) m <<= 1;
     for (uint32_t i = n + threadIdx.x; i < m; i += kThreads) list[i] = DESC ? 0 : ~0ull;
     __syncthreads();
-    auto step = [&](uint32_t size, uint32_t stride) {
-        for (uint32_t t = threadIdx.x; t < m / 2; t += kThreads) {
-            const uint32_t i = 2 * t - (t & (stride - 1)), j = i + stride;
-            const u64 x = list[i], y = list[j];
-            const bool up = ((i & size) != 0) == DESC;
-            if (x != y && (x > y) == up) list[i] = y, list[j] = x;
-        }
-    };
+#pragma unroll 1
     for (uint32_t size = 2; size <= m; size <<= 1) {
-        uint32_t stride = size / 2;
-        if (stride > 64) {
-            __syncthreads();
-            for (; stride > 64; stride >>= 1) {
-                step(size, stride);
-                __syncthreads();
+#pragma unroll 1
+        for (uint32_t stride = size / 2; stride > 0; stride >>= 1) {
+            for (uint32_t t = threadIdx.x; t < m / 2; t += kThreads) {
+                const uint32_t i = 2 * t - (t & (stride - 1)), j = i + stride;
+                const u64 x = list[i], y = list[j];
+                const bool up = ((i & size) != 0) == DESC;
+                if (x != y && (x > y) == up) list[i] = y, list[j] = x;
             }
-        }
-        for (; stride > 0; stride >>= 1) {
-            step(size, stride);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            // a wave's pairs at strides up to 64 are its own: the block meets where the next stride or size needs it
+            if (stride > 64 || (stride == 1 && size >= 128)) __syncthreads();
+            else {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
         }
     }
     __syncthreads();
-}
-
-// Gathers the elements of `in` with klo <= key <= khi into the list.  False: there are more than fit.
-template <typename T>
-__device__ __forceinline__ bool gather(const SampleArgs& a, const T* row, const Border& in, uint32_t klo, uint32_t khi, Shared& sh) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.n_list = 0;
-    __syncthreads();
-    each_element(row, 0, a.V, threadIdx.x, kThreads, [&](float l, uint32_t i) {
-        const uint32_t key = key_of(l);
-        if (!candidate(l) || key < klo || key > khi || !inside(in, key, i)) return;
-        const uint32_t at = atomicAdd(&sh.n_list, 1u);
-        if (at < kList) sh.list[at] = entry(key, i);
-    });
-    __syncthreads();
-    return sh.n_list <= kList;
 }
 
 // The place in the list's first n entries (sorted) at which their running mass reaches `target`.
 __device__ __forceinline__ uint32_t place_of_mass(const Row& r, uint32_t n, u64 target, Shared& sh) {
-    u64 carry = 0, all;
-    __syncthreads();
-    if (threadIdx.x == 0) sh.at = n - 1;
-    for (uint32_t i0 = 0; i0 < n; i0 += kThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        const u64 w = i < n ? weight(r, entry_value(sh.list[i]), sh.tab) : 0;
-        const u64 upto = carry + block_incl(w, sh, &all);
-        if (i < n && upto >= target && upto - w < target) sh.at = i;
-        carry += all;
-    }
-    __syncthreads();
-    return sh.at;
-}
-
-// The index of the rank-th element with this key, by counts of tiles (rank >= 1, and there are that many).
-template <typename T>
-__device__ __forceinline__ uint32_t index_of_rank(const SampleArgs& a, const T* row, const Border& in, uint32_t key, u64 rank, Shared& sh) {
-    const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __syncthreads();
-    for (uint32_t t = tiles + threadIdx.x; t < kTiles; t += kThreads) sh.ties[t] = 0;
-    for (uint32_t t = wave; t < tiles; t += kWaves) {
-        uint32_t n = 0;
-        each_element(row, t * a.tile, std::min(a.V, (t + 1) * a.tile), lane, 64,
-                     [&](float l, uint32_t i) { n += candidate(l) && key_of(l) == key && inside(in, key, i); });
-        for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
-        if (lane == 0) sh.ties[t] = n;
-    }
-    __syncthreads();
-    u64 n[kPer], sum = 0, all;
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) n[q] = sh.ties[kPer * threadIdx.x + q], sum += n[q];
-    u64 upto = block_incl(sum, sh, &all) - sum;
+    u64 v[kPer];
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-        if (upto < rank && rank <= upto + n[q]) sh.bin = kPer * threadIdx.x + q, sh.above = upto;
-        upto += n[q];
+        const uint32_t i = kPer * threadIdx.x + q;
+        v[q] = i < n ? weight(r, entry_value(sh.list[i]), sh.tab) : 0;
     }
-    __syncthreads();
-    if (wave == 0) {
-        const uint32_t t = sh.bin, end = std::min(a.V, (t + 1) * a.tile);
-        uint32_t left = (uint32_t)(rank - sh.above);
-        for (uint32_t i0 = t * a.tile; i0 < end; i0 += 64) {
-            const uint32_t i = i0 + lane;
-            const float l = i < end ? (float)row[i] : __builtin_nanf("");
-            const bool tie = candidate(l) && key_of(l) == key && inside(in, key, i);
-            const u64 ties = __ballot(tie);
-            const uint32_t here = __popcll(ties);
-            if (here < left) {
-                left -= here;
-                continue;
-            }
-            if (tie && __popcll(ties & ((1ull << lane) - 1)) == left - 1) sh.at = i;
-            break;
-        }
-    }
-    __syncthreads();
-    return sh.at;
-}
-
-// The border of the share / count `need` (> 0) of the elements with klo <= key <= khi inside `in`.
-template <typename T, Kind KIND>
-__device__ __forceinline__ Border border_in(const SampleArgs& a, const T* row, const Row& r, const Border& in, uint32_t klo, uint32_t khi, u64 need,
-                            Shared& sh) {
-    while (!gather(a, row, in, klo, khi, sh)) {
-        if (klo == khi) {
-            u64 rank = need;
-            if (KIND == kMass) {
-                const u64 w = weight(r, value_of(khi), sh.tab);
-                rank = w ? (need + w - 1) / w : 1;
-            }
-            const u64 n = sh.n_list;
-            return Border{khi, index_of_rank(a, row, in, khi, rank < n ? rank : n, sh)};
-        }
-        const int bits = 32 - __clz(khi - klo), shift = bits > 12 ? bits - 12 : 0;      // 2^12 = kBins ranges
-        histogram<T, KIND, true>(a, row, r, in, klo, khi, shift, sh);
-        find_bin<KIND>(need, -1.0, sh);
-        need -= sh.above;
-        khi -= sh.bin << shift;
-        const uint32_t width = (1u << shift) - 1;
-        klo = khi - klo > width ? khi - width : klo;
-    }
-    const uint32_t n = sh.n_list;
-    sort_list<true>(n, sh.list);
-    const u64 x = sh.list[KIND == kMass ? place_of_mass(r, n, need, sh) : (uint32_t)std::min<u64>(need, n) - 1];
-    __syncthreads();
-    return Border{(uint32_t)(x >> 32), ~(uint32_t)x};
-}
-
-__device__ __forceinline__ u64 share_of(double p, u64 total) {
-    const u64 t = (u64)ceil((p > 0.0 ? p : 0.0) * (double)total);
-    return t < 1 ? 1 : t > total ? total : t;
+    find_place(v, target, 0, sh);
+    return std::min(sh.bin, n - 1);
 }
 
 __device__ __forceinline__ u64 draw_target(const SampleArgs& a, int64_t at, u64 total) {
@@ -455,9 +376,12 @@ __device__ __forceinline__ u64 draw_target(const SampleArgs& a, int64_t at, u64 
     const double t = u > 0.0 ? u * (double)total : 0.0;             // NaN counts as 0
     return t < (double)total ? std::min<u64>((u64)t, total - 1) : total - 1;
 }
-__device__ __forceinline__ void put_draw(const SampleArgs& a, const Row& r, int64_t at, uint32_t i, float l, u64 total) {
+__device__ __forceinline__ void put_draw(const SampleArgs& a, const Row& r, int64_t at, uint32_t i, float l, u64 total, const double* tab) {
     a.ids[at] = i;
-    a.probs[at] = (float)(ldexp(exp(log_weight(r, l)), r.scale) / (double)total);
+    a.probs[at] = (float)(weight_units(r, l, tab) / (double)total);
+}
+__device__ __forceinline__ void draw_nothing(const SampleArgs& a, int64_t b) {
+    for (int q = threadIdx.x; q < a.draws; q += kThreads) a.ids[b * a.draws + q] = -1, a.probs[b * a.draws + q] = 0.f;
 }
 
 // The draws of a row whose first top_k elements (all, where that is off) are among the list's n entries.
@@ -467,14 +391,10 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, const Row& r
         sort_list<true>(n, sh.list);
         if (r.k > 0 && r.k < n) keep = (uint32_t)r.k;
     }
-    u64 all;
     if (r.p < 1.0) {
-        u64 total = 0;
-        for (uint32_t i0 = 0; i0 < keep; i0 += kThreads) {
-            const uint32_t i = i0 + threadIdx.x;
-            block_incl(i < keep ? weight(r, entry_value(sh.list[i]), sh.tab) : 0, sh, &all);
-            total += all;
-        }
+        u64 sum = 0, total;
+        for (uint32_t i = threadIdx.x; i < keep; i += kThreads) sum += weight(r, entry_value(sh.list[i]), sh.tab);
+        block_incl(sum, sh, &total);
         keep = place_of_mass(r, keep, share_of(r.p, total), sh) + 1;
     }
     // the kept entries in index order, with their running sums (below min_p: weight zero)
@@ -483,18 +403,17 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, const Row& r
         sh.list[i] = ((u64)(~(uint32_t)x) << 32) | (uint32_t)(x >> 32);
     }
     sort_list<false>(keep, sh.list);
-    u64 total = 0;
-    for (uint32_t i0 = 0; i0 < keep; i0 += kThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        u64 w = 0;
-        if (i < keep) {
-            const float l = value_of((uint32_t)sh.list[i]);
-            if (log_weight(r, l) >= r.log_min_p) w = weight(r, l, sh.tab);
-        }
-        const u64 upto = total + block_incl(w, sh, &all);
-        if (i < keep) sh.run[i] = upto;
-        total += all;
+    u64 v[kPer], sum = 0, total;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const uint32_t i = kPer * threadIdx.x + q;
+        const float l = i < keep ? value_of((uint32_t)sh.list[i]) : -__builtin_inff();
+        v[q] = i < keep && passes(r, l) ? weight(r, l, sh.tab) : 0;
+        sum += v[q];
     }
+    u64 upto = block_incl(sum, sh, &total) - sum;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) upto += v[q], sh.run[kPer * threadIdx.x + q] = upto;
     __syncthreads();
     for (int q = threadIdx.x; q < a.draws; q += kThreads) {
         const u64 want = draw_target(a, b * a.draws + q, total);
@@ -505,231 +424,546 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, const Row& r
             else lo = mid + 1;
         }
         const u64 x = sh.list[lo];
-        put_draw(a, r, b * a.draws + q, (uint32_t)(x >> 32), value_of((uint32_t)x), total);
+        put_draw(a, r, b * a.draws + q, (uint32_t)(x >> 32), value_of((uint32_t)x), total, sh.tab);
     }
 }
 
-// The draws by the sums of the row's tiles in sh.tile (zero past the last): one wave a draw.
+// ------------------------------------------------------------------------------- looks at the elements
+// Adds one to *n and puts x at that place of the list, if it has one.
+__device__ __forceinline__ void append(u64 x, u64* list, uint32_t* n) {
+    const uint32_t at = atomicAdd(n, 1u);
+    if (at < kBins) list[at] = x;
+}
+
 template <typename T>
-__device__ __forceinline__ void draw_from_tiles(const SampleArgs& a, const T* row, const Row& r, const Border& in, int64_t b, Shared& sh) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    u64 w[kPer], sum = 0, total;
-    __syncthreads();
+__device__ __forceinline__ float look_max(const T* row, uint32_t lo, uint32_t hi) {
+    float top = -__builtin_inff();
+    each_element<8>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) w[q] = sh.tile[kPer * threadIdx.x + q], sum += w[q];
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, l[e]);          // fmaxf drops NaN
+    });
+    return top;
+}
+
+// Elements from klo on, into the list.
+template <typename T>
+__device__ __forceinline__ void look_gather(const T* row, uint32_t lo, uint32_t hi, uint32_t klo, u64* list, uint32_t* n) {
+    const float from = value_of(klo);                                // a candidate: NaN and -infinity fail the comparison
+    each_element<8>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t i) {
+        if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= from) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (l[e] >= from) append(entry(key_of(l[e]), i + e), list, n);
+        }
+    });
+}
+
+// Masses by bins of l in sh.bins, which the caller has cleared; returns the thread's sum of all its weights.
+template <typename T>
+__device__ __forceinline__ u64 look_bins(const T* row, uint32_t lo, uint32_t hi, const Row& r, Shared& sh) {
+    u64 sum = 0;
+    each_element<4>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
+        u64 w[4];
+        int bin[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {                                // all four without a branch: their steps overlap
+            w[e] = weight(r, l[e], sh.tab);                          // zero for what is no candidate
+            bin[e] = bin_of(r, l[e]);
+            sum += w[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (bin[e] < kBins) atomicAdd(&sh.bins[bin[e]], w[e]);
+    });
+    return sum;
+}
+
+// Counts (MASS: masses) of the keys klo to khi by ranges of 2^shift below khi, in sh.bins.
+template <typename T, bool MASS>
+__device__ __forceinline__ void look_ranges(const T* row, uint32_t V, const Row& r, uint32_t klo, uint32_t khi, int shift, Shared& sh) {
+    for (int q = 0; q < kPer; ++q) sh.bins[q * kThreads + threadIdx.x] = 0;
+    __syncthreads();
+    each_element<4>(row, 0, V, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t key = key_of(l[e]);
+            if (candidate(l[e]) && key >= klo && key <= khi)
+                atomicAdd(&sh.bins[(khi - key) >> shift], MASS ? weight(r, l[e], sh.tab) : 1);
+        }
+    });
+    __syncthreads();
+}
+
+// bfloat16 values with a counter, in descending order of the value: their place, and the value of a place.
+__device__ __forceinline__ uint32_t place_of_value(uint32_t d, int32_t sign) { return d ^ (uint32_t)(2047 - sign); }      // sign 0 or -1
+__device__ __forceinline__ float value_of_place(uint32_t place) {
+    const uint32_t d = place < 2048 ? 2047 - place : place - 2048;
+    return __uint_as_float(((d + kFirstMag) << 16) | (place < 2048 ? 0u : 0x80000000u));
+}
+// Counts by value in sh.count, which the caller has cleared; candidates without a counter go to the list.
+__device__ __forceinline__ void look_values(const __bf16* row, uint32_t lo, uint32_t hi, Shared& sh) {
+    each_element<8>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t u = __float_as_uint(l[e]), d = ((u >> 16) & 0x7fffu) - kFirstMag;
+            if (d < 2048) atomicAdd(&sh.count[place_of_value(d, (int32_t)u >> 31)], 1u);
+            else if (candidate(l[e])) append(entry(key_of(l[e]), i + e), sh.list, &sh.n_list);
+        }
+    });
+}
+
+// Tile by tile of [t0, t1): the weights above khi that pass min_p, and of the elements from klo to khi the count (TIES) or
+// the entries in the list.
+template <typename T>
+__device__ __forceinline__ void look_tiles(const SampleArgs& a, const T* row, const State& st, uint32_t t0, uint32_t t1, const double* tab,
+                                           u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Row r = st.r;
+    const uint32_t klo = st.klo, khi = st.khi;
+    const bool count = st.ties;
+    for (uint32_t t = t0 + wave; t < t1; t += kWaves) {
+        u64 w = 0;
+        uint32_t n = 0;
+        each_element<4>(row, t * a.tile, std::min(a.V, (t + 1) * a.tile), lane, 64, [&](const float(&l)[4], uint32_t i) {
+            bool kept[4];
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t key = key_of(l[e]);
+                const bool in = candidate(l[e]) && key >= klo;
+                kept[e] = in && key > khi;
+                any |= kept[e];
+                if (in && !kept[e]) {
+                    if (count) ++n;
+                    else append(entry(key, i + e), list, n_list);
+                }
+            }
+            if (any) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const u64 x = weight(r, l[e], tab);
+                    w += kept[e] && passes(r, l[e]) ? x : 0;
+                }
+            }
+        });
+        w = wave_incl(w);
+        if (lane == 63) tile[t] = w;
+        if (count) {
+            const u64 c = wave_incl(n);
+            if (lane == 63) ties[t] = (uint32_t)c;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------- borders
+// The keys of a bin: [first, last]; every wave searches for itself, 64 keys at a time.
+__device__ __forceinline__ void keys_of_bin(const Row& r, int bin, uint32_t* first, uint32_t* last) {
+    uint32_t end[2];
+#pragma unroll 1
+    for (int s = 0; s < 2; ++s) {                                    // the largest key with bin_of >= bin + s
+        uint32_t lo = kLowestKey - 1, hi = r.top + 1;                // holds at lo, not at hi
+        if (bin + s <= 0) lo = hi - 1;
+        if (bin + s > kBins) hi = lo + 1;
+#pragma unroll 1
+        while (hi - lo > 1) {
+            const uint32_t step = (hi - lo - 1) / 64 + 1;
+            const u64 at = (u64)lo + (u64)step * ((threadIdx.x & 63) + 1);
+            const bool yes = at < hi && bin_of(r, value_of((uint32_t)at)) >= bin + s;
+            const int n = __popcll(__ballot(yes));
+            const u64 next = (u64)lo + (u64)step * (n + 1);
+            lo += step * n;
+            hi = next < hi ? (uint32_t)next : hi;
+        }
+        end[s] = lo;
+    }
+    *last = end[0];
+    *first = end[1] + 1;
+}
+
+// The lowest key that the gather needs: of the bin in which the k-th largest of the groups' maxima lies (0: below the bins).
+__device__ __forceinline__ uint32_t key_by_maxima(const Row& r, int groups, Shared& sh) {
+    for (int q = 0; q < kPer; ++q) sh.count[q * kThreads + threadIdx.x] = 0;
+    __syncthreads();
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+        const float m = sh.group[g];
+        const int b = candidate(m) ? bin_of(r, m) : kBins;
+        if (b < kBins) atomicAdd(&sh.count[b], 1u);
+    }
+    __syncthreads();
+    u64 v[kPer];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) v[q] = sh.count[kPer * threadIdx.x + q];
+    find_place(v, (u64)r.k, 0, sh);
+    uint32_t first = 0, last;
+    if (sh.bin < kBins) keys_of_bin(r, sh.bin, &first, &last);
+    return first;
+}
+
+// Narrows the keys klo to khi, which hold the border, to its own key; *need becomes the number of that key's elements that
+// are kept.  MASS: it comes in as units of mass.
+template <typename T, bool MASS>
+__device__ __forceinline__ void narrow(const SampleArgs& a, const T* row, const Row& r, uint32_t klo, uint32_t* khi, u64* need, Shared& sh) {
+#pragma unroll 1
+    do {
+        const int bits = klo == *khi ? 0 : 32 - __clz(*khi - klo), shift = bits > 12 ? bits - 12 : 0;      // 2^12 = kBins ranges
+        look_ranges<T, MASS>(row, a.V, r, klo, *khi, shift, sh);
+        u64 v[kPer];
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) v[q] = sh.bins[kPer * threadIdx.x + q];
+        find_place(v, *need, 0, sh);
+        *need -= sh.above;
+        *khi -= sh.bin << shift;
+        const uint32_t width = (1u << shift) - 1;
+        klo = *khi - klo > width ? *khi - width : klo;
+        __syncthreads();
+    } while (klo < *khi);
+    if (MASS) {
+        const u64 w = weight(r, value_of(*khi), sh.tab);
+        *need = w ? (*need + w - 1) / w : 1;
+    }
+}
+
+// sh.bins holds the masses by bins, sh.rest what lies lower: the border of top_p (of the mass `of`; 0: all) for look_tiles.
+__device__ __forceinline__ void border_by_bins(State& st, u64 of, Shared& sh) {
+    u64 v[kPer], all, sum = 0;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) v[q] = sh.bins[kPer * threadIdx.x + q], sum += v[q];
+    block_incl(sum, sh, &all);
+    const u64 target = share_of(st.r.p, of ? of : all + sh.rest);
+    find_place(v, target, 0, sh);
+    st.need = target - sh.above;
+    keys_of_bin(st.r, sh.bin, &st.klo, &st.khi);
+    st.ties = 0;
+    st.mode = kTiles;
+    __syncthreads();
+}
+
+// sh.count holds the counts by value, the list the n others: the border of top_k and top_p for look_tiles.
+__device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st, uint32_t n, Shared& sh) {
+    uint32_t c[kPer];
+    float top = -__builtin_inff(), l[kPer];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        c[q] = sh.count[kPer * threadIdx.x + q];
+        l[q] = value_of_place(kPer * threadIdx.x + q);
+        top = c[q] ? fmaxf(top, l[q]) : top;
+    }
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) top = fmaxf(top, entry_value(sh.list[i]));
+    top = block_max(top, sh);
+    Row& r = st.r;
+    st.mode = kDone;
+    st.klo = 1, st.khi = 0;                                          // none: every key lies above
+    st.ties = 1;
+    st.need = 0;
+    if (!candidate(top)) return;
+    st.mode = kTiles;
+    const float by = (float)(1.4426950408889634 * r.inv_t);
+    float mass = 0.f;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) mass += c[q] ? (float)c[q] * (l[q] == top ? 1.f : __builtin_amdgcn_exp2f((l[q] - top) * by)) : 0.f;
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        const float x = entry_value(sh.list[i]);
+        mass += x == top ? 1.f : __builtin_amdgcn_exp2f((x - top) * by);
+    }
+    mass = block_sum(mass, sh);
+    set_scale(r, top, fminf(mass * 1.01f + 1.f, (float)a.V));
+    if (r.k == 0 && !(r.p < 1.0)) return;
+    // in descending order: the list above the counters' range, the positive values, the list between, the negative, the rest
+    const float high = value_of_place(0), low = value_of_place(kBins - 1);
+    u64 w[kPer];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) w[q] = c[q] ? weight(r, l[q], sh.tab) : 0;
+    u64 of = 0;
+#pragma unroll 1
+    for (int pass = r.k > 0 ? 0 : 1; pass < (r.p < 1.0 ? 2 : 1); ++pass) {           // by count, then by mass
+        u64 v[kPer], zone[3] = {0, 0, 0}, sum = 0, all;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) v[q] = pass ? w[q] * c[q] : c[q], sum += v[q];
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const float x = entry_value(sh.list[i]);
+            const u64 one = pass ? weight(r, x, sh.tab) : 1;
+            const int at = x > high ? 0 : x < low ? 2 : 1;
+            zone[0] += at == 0 ? one : 0;
+            zone[1] += at == 1 ? one : 0;
+            zone[2] += at == 2 ? one : 0;
+        }
+        block_incl(sum, sh, &all);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) block_incl(zone[q], sh, &zone[q]);
+        const u64 total = all + zone[0] + zone[1] + zone[2];
+        if (pass == 0 && (u64)r.k >= total) continue;
+        const u64 target = pass ? share_of(r.p, of ? of : total) : (u64)r.k;
+        uint32_t place = kBins;
+        if (target > zone[0]) {
+            find_place(v, target - zone[0], zone[1], sh);
+            place = sh.bin;
+        }
+        if (place < kBins) {
+            const u64 need = target - zone[0] - sh.above;
+            const float x = value_of_place(place);
+            const u64 one = weight(r, x, sh.tab);
+            st.klo = st.khi = key_of(x);
+            st.need = pass ? (need + one - 1) / one : need;          // a place found by mass has weight
+            // the mass of the first k, for top_p: all above the place, and need of it
+            if (pass == 0) {
+                u64 above = 0;
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) above += kPer * threadIdx.x + q < place ? w[q] * c[q] : 0;
+                for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+                    const float y = entry_value(sh.list[i]);
+                    above += y > x ? weight(r, y, sh.tab) : 0;
+                }
+                block_incl(above, sh, &of);
+                of += need * one;
+            }
+        } else {                                                     // among the list's entries, one by one
+            st.mode = kAlone;
+            return;
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------- the end of a row
+// The tiles' sums and the border (ties or list entries) are in LDS: adds the border's kept elements to their tiles, and
+// draws.  False: the list has overflown.
+template <typename T>
+__device__ __forceinline__ bool draw_from_tiles(const SampleArgs& a, const T* row, const State& st, int64_t b, Shared& sh) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Row r = st.r;
+    const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
+    uint32_t last_key = 0, last_idx = 0;                             // kept are the keys above, and that key up to the index
+    __syncthreads();
+    if (st.ties && st.need) {
+        u64 v[kPer];
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+            const uint32_t t = kPer * threadIdx.x + q;
+            v[q] = t < tiles ? sh.ties[t] : 0;
+        }
+        find_place(v, st.need, 0, sh);
+        const uint32_t t = sh.bin;                                   // the tile of the last kept
+        const float l = value_of(st.khi);
+        const u64 one = passes(r, l) ? weight(r, l, sh.tab) : 0;
+        uint32_t left = (uint32_t)(st.need - sh.above);
+        for (uint32_t i = threadIdx.x; i <= t && i < tiles; i += kThreads) sh.tile[i] += one * (i < t ? sh.ties[i] : left);
+        if (wave == 0) {
+            const uint32_t end = std::min(a.V, (t + 1) * a.tile);
+            for (uint32_t i0 = t * a.tile; i0 < end; i0 += 64) {
+                const uint32_t i = i0 + lane;
+                const float x = i < end ? (float)row[i] : __builtin_nanf("");
+                const bool tie = candidate(x) && key_of(x) == st.khi;
+                const u64 all = __ballot(tie);
+                const uint32_t here = __popcll(all);
+                if (here < left) {
+                    left -= here;
+                    continue;
+                }
+                if (tie && __popcll(all & ((1ull << lane) - 1)) == left - 1) sh.at = i;
+                break;
+            }
+        }
+        __syncthreads();
+        last_key = st.khi;
+        last_idx = sh.at;
+    } else if (!st.ties) {
+        const uint32_t n = sh.n_list;
+        if (n > kBins) return false;
+        sort_list<true>(n, sh.list);
+        const uint32_t last = place_of_mass(r, n, st.need, sh);
+        for (uint32_t i = threadIdx.x; i <= last; i += kThreads) {
+            const u64 y = sh.list[i];
+            const float l = entry_value(y);
+            if (passes(r, l)) atomicAdd(&sh.tile[~(uint32_t)y / a.tile], weight(r, l, sh.tab));
+        }
+        last_key = (uint32_t)(sh.list[last] >> 32);
+        last_idx = ~(uint32_t)sh.list[last];
+        __syncthreads();
+    }
+    u64 w[kPer], sum = 0, total;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const uint32_t t = kPer * threadIdx.x + q;
+        w[q] = t < tiles ? sh.tile[t] : 0;
+        sum += w[q];
+    }
     u64 upto = block_incl(sum, sh, &total) - sum;
 #pragma unroll
     for (int q = 0; q < kPer; ++q) upto += w[q], sh.tile[kPer * threadIdx.x + q] = upto;
     __syncthreads();
     for (int q = wave; q < a.draws; q += kWaves) {
         const u64 want = draw_target(a, b * a.draws + q, total);
-        uint32_t lo = 0, hi = kTiles - 1;
+        uint32_t lo = 0, hi = tiles - 1;
         while (lo < hi) {
             const uint32_t mid = (lo + hi) / 2;
             if (sh.tile[mid] > want) hi = mid;
             else lo = mid + 1;
         }
         u64 before = lo ? sh.tile[lo - 1] : 0;
-        const uint32_t end = std::min(a.V, (lo + 1) * a.tile);
-        for (uint32_t i0 = lo * a.tile; i0 < end; i0 += 256) {
-            float v[4];
+        bool found = false;
+        each_element<4>(row, lo * a.tile, std::min(a.V, (lo + 1) * a.tile), lane, 64, [&](const float(&l)[4], uint32_t i) {
+            if (found) return;
             u64 x[4], four = 0;
-            const uint32_t i = i0 + 4 * lane;
-            load4(row, i, end, v);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = kept_weight(r, in, v[e], i + e, sh.tab), four += x[e];
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t key = key_of(l[e]);
+                const bool kept = candidate(l[e]) && (key > last_key || (key == last_key && i + e <= last_idx)) && passes(r, l[e]);
+                const u64 one = weight(r, l[e], sh.tab);
+                x[e] = kept ? one : 0;
+                four += x[e];
+            }
             const u64 sums = before + wave_incl(four);
             const u64 hit = __ballot(sums > want);
+            before = lane64(sums, 63);
             if (hit) {
+                found = true;
                 if (lane == __ffsll((long long)hit) - 1) {
                     u64 at = sums - four;
-                    int e = 0;
-                    for (; e < 3; ++e) {
-                        at += x[e];
-                        if (at > want) break;
-                    }
-                    float l = v[0];
+                    float l0 = l[0];
+                    uint32_t e0 = 0;
+                    bool past = false;
 #pragma unroll
-                    for (int g = 1; g < 4; ++g) l = e == g ? v[g] : l;
-                    put_draw(a, r, b * a.draws + q, i + e, l, total);
+                    for (int e = 0; e < 4; ++e) {
+                        at += x[e];
+                        if (!past) l0 = l[e], e0 = e;
+                        past |= at > want;
+                    }
+                    put_draw(a, r, b * a.draws + q, i + e0, l0, total, sh.tab);
                 }
-                break;
             }
-            before = ((u64)__shfl((uint32_t)(sums >> 32), 63) << 32) | __shfl((uint32_t)sums, 63);
-        }
+        });
     }
-}
-
-__device__ __forceinline__ void draw_nothing(const SampleArgs& a, int64_t b) {
-    for (int q = threadIdx.x; q < a.draws; q += kThreads) a.ids[b * a.draws + q] = -1, a.probs[b * a.draws + q] = 0.f;
-}
-
-// ------------------------------------------------------------------------------- a row's settings
-__device__ __forceinline__ Row settings(const SampleArgs& a, int64_t b) {
-    double t = a.temperature ? (double)a.temperature[b] : a.t;
-    const double p = a.top_p ? (double)a.top_p[b] : a.p, mp = a.min_p ? (double)a.min_p[b] : a.mp;
-    Row r;
-    r.k = a.top_k ? a.top_k[b] : a.k;
-    if (!(t > 0.0) || t > 3e38) t = 1.0, r.k = 1;
-    if (r.k < 0 || r.k >= a.V) r.k = 0;
-    r.p = p < 1.0 ? p : 1.0;
-    r.inv_t = 1.0 / t;
-    r.log_min_p = mp > 0.0 ? log(mp < 1.0 ? mp : 1.0) : -__builtin_inf();
-    r.step = 184.6649652337873 * r.inv_t;                            // 128 / ln 2
-    r.lmax = 0.f;
-    r.scale = 0;
-    r.cut = 0.0;
-    r.bin_scale = (float)((double)kBins / (double)kRange * r.inv_t);
-    return r;
-}
-// Whether the k-th largest of `groups` maxima leads to a list: groups * ln(groups / (groups - k)) <= 1.7 groups elements
-// reach it where the groups are alike.
-__device__ __forceinline__ bool by_maxima(const Row& r, int64_t groups) { return r.k > 0 && 5 * r.k <= 4 * groups; }
-
-// The maximum, the scale (the row's mass, at most `most` times the largest weight, has to fit 62 bits), and for top_p the
-// range of the bins: V elements below it weigh less than half of what top_p leaves out of a mass of at least `least`.
-__device__ __forceinline__ void set_scale(const SampleArgs& a, Row& r, float lmax, float least, float most) {
-    r.lmax = lmax;
-    int ex;
-    (void)frexpf(most, &ex);                                         // most < 2^ex
-    r.scale = min(51, 62 - ex);
-    r.cut = -128.0 * (double)(r.scale + 2);
-    float range = kRange;
-    if (r.k == 0 && r.p < 1.0) {
-        const float out = (float)(1.0 - r.p) * least * 0.75f;
-        const float down = logf(2.f * (float)a.V / out);
-        range = out > 0.f && down < kRange ? fmaxf(down, 0.125f) : kRange;
-    }
-    r.bin_scale = (float)((double)kBins / (double)range * r.inv_t);
+    return true;
 }
 
 // ------------------------------------------------------------------------------- one block, one row
-// Counts the maxima (threads' own groups) into bins and gathers what reaches the k-th largest.  False: more than the list
-// holds, or the k-th largest lies below the bins.
-__device__ __forceinline__ uint32_t key_by_maxima(const Row& r, const float* maxima, uint32_t groups, Shared& sh) {
-    for (int b = threadIdx.x; b < kBins; b += kThreads) sh.count[b] = 0;
-    if (threadIdx.x == 0) sh.rest = 0;
-    __syncthreads();
-    for (uint32_t g = threadIdx.x; g < groups; g += kThreads) {
-        const float m = maxima[g];
-        const int b = candidate(m) ? bin_of(r, m) : kBins;
-        if (b < kBins) atomicAdd(&sh.count[b], 1u);
-    }
-    __syncthreads();
-    find_bin<kCount>((u64)r.k, -1.0, sh);
-    return sh.bin < kBins ? first_key_of_bin(r, sh.bin) : 0;
-}
-
-// The sums over the row's tiles (sh.tile) of the weights inside `in`; BORDER: of those above khi alone, the ones from klo to
-// khi go to the list, false when they do not fit.
-template <typename T, bool BORDER>
-__device__ __forceinline__ bool sum_tiles(const SampleArgs& a, const T* row, const Row& r, const Border& in, uint32_t klo,
-                                          uint32_t khi, Shared& sh) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
+template <typename T>
+__device__ __forceinline__ void look_tiles_alone(const SampleArgs& a, const T* row, const State& st, Shared& sh) {
     __syncthreads();
     if (threadIdx.x == 0) sh.n_list = 0;
-    for (uint32_t t = tiles + threadIdx.x; t < kTiles; t += kThreads) sh.tile[t] = 0;
     __syncthreads();
-    for (uint32_t t = wave; t < tiles; t += kWaves) {
-        u64 w = 0;
-        each_element(row, t * a.tile, std::min(a.V, (t + 1) * a.tile), lane, 64, [&](float l, uint32_t i) {
-            if constexpr (BORDER) {
-                const uint32_t key = key_of(l);
-                if (!candidate(l) || key < klo || !inside(in, key, i)) return;
-                if (key <= khi) {
-                    const uint32_t at = atomicAdd(&sh.n_list, 1u);
-                    if (at < kList) sh.list[at] = entry(key, i);
-                    return;
-                }
-            }
-            w += kept_weight(r, in, l, i, sh.tab);
-        });
-        w = wave_incl(w);
-        if (lane == 63) sh.tile[t] = w;
-    }
+    look_tiles(a, row, st, 0, (a.V + a.tile - 1) / a.tile, sh.tab, sh.tile, sh.ties, sh.list, &sh.n_list);
     __syncthreads();
-    return sh.n_list <= kList;
 }
 
+// The row by looks for any type; what the lists of the quick ways cannot hold ends here too (quick false).
 template <typename T>
-__device__ __forceinline__ void whole_row(const SampleArgs& a, int64_t b, Shared& sh) {
+__device__ __forceinline__ void row_by_bins(const SampleArgs& a, int64_t b, bool quick, Shared& sh) {
     const T* row = (const T*)a.logits + b * a.ld;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Row r = settings(a, b);
-    Border in = {0, 0};                                              // key 0 is below every candidate: all are inside
-    const float own = thread_max(row, 0, a.V, threadIdx.x, kThreads);
-    float top = own;
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (lane == 0) sh.wmax[wave] = top;
-    __syncthreads();
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, sh.wmax[i]);
+    State st;
+    st.r = settings(a, b);
+    Row& r = st.r;
+    const float own = look_max(row, 0, a.V);
+    const float top = block_max(own, sh);
     if (!candidate(top)) return draw_nothing(a, b);
-    if (a.V <= kSmall || by_maxima(r, kThreads)) {
-        set_scale(a, r, top, 1.f, (float)kList);
-        uint32_t klo = kLowestKey;
-        if (a.V > kSmall) {
-            sh.group[threadIdx.x] = own;
-            klo = key_by_maxima(r, sh.group, kThreads, sh);
+    if (quick && by_maxima(r, kThreads)) {
+        set_scale(r, top, (float)kBins);
+        set_bins(r, kRange);
+        if (threadIdx.x == 0) sh.n_list = 0;
+        sh.group[threadIdx.x] = own;
+        const uint32_t klo = key_by_maxima(r, kThreads, sh);
+        if (klo) {
+            look_gather(row, 0, a.V, klo, sh.list, &sh.n_list);
+            __syncthreads();
+            if (sh.n_list <= kBins) return draw_from_list(a, r, b, sh.n_list, sh);
         }
-        if (klo && gather(a, row, in, klo, 0xffffffffu, sh)) return draw_from_list(a, r, b, sh.n_list, sh);
     }
     // the maxima of the threads bound the mass from below and, as often as a thread has elements, from above
-    {
-        const float c = (float)(1.4426950408889634 * r.inv_t);
-        float sum = own == top ? 1.f : candidate(own) ? __builtin_amdgcn_exp2f((own - top) * c) : 0.f;
-        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-        __syncthreads();
-        if (lane == 0) sh.wmax[wave] = sum;
-        __syncthreads();
-        sum = 0.f;
-        for (int i = 0; i < kWaves; ++i) sum += sh.wmax[i];
-        set_scale(a, r, top, sum * 0.99f, sum * 1.01f * 4.f * (float)((a.V + 4 * kThreads - 1) / (4 * kThreads)));
-    }
+    const float by = (float)(1.4426950408889634 * r.inv_t);
+    const float least = 0.99f * block_sum(own == top ? 1.f : candidate(own) ? __builtin_amdgcn_exp2f((own - top) * by) : 0.f, sh);
+    set_scale(r, top, 1.03f * least * 4.f * (float)((a.V + 4 * kThreads - 1) / (4 * kThreads)));
+    st.klo = 1, st.khi = 0;
+    st.ties = 1;
+    st.need = 0;
+    u64 of = 0;
     if (r.k > 0) {
-        histogram<T, kCount, false>(a, row, r, in, 0, 0, 0, sh);
-        find_bin<kCount>((u64)r.k, -1.0, sh);
-        const u64 above = sh.above, here = sh.in_bin, total = sh.total;
-        const int bin = sh.bin;
-        const uint32_t klo = (u64)r.k >= total ? kLowestKey : first_key_of_bin(r, bin);
-        if (std::min(above + here, total) <= kList) {
-            gather(a, row, in, klo, 0xffffffffu, sh);
-            return draw_from_list(a, r, b, sh.n_list, sh);
-        }
-        if ((u64)r.k < total) in = border_in<T, kCount>(a, row, r, in, klo, last_key_of_bin(r, bin), (u64)r.k - above, sh);
-    }
-    bool summed = false;
-    if (r.p < 1.0) {
-        histogram<T, kMass, false>(a, row, r, in, 0, 0, 0, sh);
-        find_bin<kMass>(0, r.p > 0.0 ? r.p : 0.0, sh);
-        const u64 need = sh.target - sh.above;
-        const int bin = sh.bin;
-        const uint32_t klo = first_key_of_bin(r, bin), khi = last_key_of_bin(r, bin);
-        summed = sum_tiles<T, true>(a, row, r, in, klo, khi, sh);
-        if (summed) {                                                // the border's bin: its kept elements join their tiles
-            const uint32_t n = sh.n_list;
-            sort_list<true>(n, sh.list);
-            const uint32_t last = place_of_mass(r, n, need, sh);
-            const u64 x = sh.list[last];
-            for (uint32_t i = threadIdx.x; i <= last; i += kThreads) {
-                const u64 y = sh.list[i];
-                const float l = entry_value(y);
-                if (log_weight(r, l) >= r.log_min_p) atomicAdd(&sh.tile[~(uint32_t)y / a.tile], weight(r, l, sh.tab));
+        uint32_t khi = r.top;
+        u64 need = (u64)r.k;
+        // at least k candidates?  narrow() may only look for a border that is there
+        u64 n = 0, all;
+        each_element<4>(row, 0, a.V, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
+            for (int e = 0; e < 4; ++e) n += candidate(l[e]);
+        });
+        block_incl(n, sh, &all);
+        if (need < all) {
+            narrow<T, false>(a, row, r, kLowestKey, &khi, &need, sh);
+            st.klo = st.khi = khi;
+            st.need = need;
+            if (r.p < 1.0) {                                         // the mass of the first k
+                u64 w = 0;
+                each_element<4>(row, 0, a.V, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
+                    for (int e = 0; e < 4; ++e) {
+                        const u64 one = weight(r, l[e], sh.tab);
+                        w += candidate(l[e]) && key_of(l[e]) > khi ? one : 0;
+                    }
+                });
+                block_incl(w, sh, &of);
+                of += need * weight(r, value_of(khi), sh.tab);
             }
-            in = Border{(uint32_t)(x >> 32), ~(uint32_t)x};
-        } else {
-            in = border_in<T, kMass>(a, row, r, in, klo, khi, need, sh);
         }
     }
-    if (!summed) sum_tiles<T, false>(a, row, r, in, 0, 0, sh);
-    draw_from_tiles(a, row, r, in, b, sh);
+    if (r.p < 1.0) {
+        set_bins(r, r.k == 0 ? range_for(r, a.V, least) : kRange);
+        __syncthreads();
+        for (int q = 0; q < kPer; ++q) sh.bins[q * kThreads + threadIdx.x] = 0;
+        __syncthreads();
+        const u64 mine = look_bins(row, 0, a.V, r, sh);
+        u64 all, in_bins, sum = 0;
+        block_incl(mine, sh, &all);
+        for (int q = 0; q < kPer; ++q) sum += sh.bins[q * kThreads + threadIdx.x];
+        block_incl(sum, sh, &in_bins);
+        if (threadIdx.x == 0) sh.rest = all - in_bins;
+        __syncthreads();
+        border_by_bins(st, of, sh);
+        look_tiles_alone(a, row, st, sh);
+        if (draw_from_tiles(a, row, st, b, sh)) return;
+        narrow<T, true>(a, row, r, st.klo, &st.khi, &st.need, sh);
+        st.klo = st.khi;
+        st.ties = 1;
+    }
+    look_tiles_alone(a, row, st, sh);
+    draw_from_tiles(a, row, st, b, sh);
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     __shared__ Shared sh;
+    const int64_t b = blockIdx.x;
     make_table(sh);
-    whole_row<T>(a, blockIdx.x, sh);
+    if (threadIdx.x == 0) sh.n_list = 0;
+    for (int q = 0; q < kPer; ++q) sh.count[q * kThreads + threadIdx.x] = 0;
+    __syncthreads();
+    const T* row = (const T*)a.logits + b * a.ld;
+    if (a.V <= kSmall) {                                             // the list, whatever the settings
+        float top = -__builtin_inff();
+        for (uint32_t i = threadIdx.x; i < a.V; i += kThreads) {
+            const float l = (float)row[i];
+            top = fmaxf(top, l);
+            if (candidate(l)) append(entry(key_of(l), i), sh.list, &sh.n_list);
+        }
+        top = block_max(top, sh);
+        if (!candidate(top)) return draw_nothing(a, b);
+        Row r = settings(a, b);
+        set_scale(r, top, (float)kSmall);
+        return draw_from_list(a, r, b, sh.n_list, sh);
+    }
+    if constexpr (sizeof(T) == 2) {
+        look_values(row, 0, a.V, sh);
+        __syncthreads();
+        if (sh.n_list <= kBins) {
+            State st;
+            st.r = settings(a, b);
+            border_by_values(a, st, sh.n_list, sh);
+            if (st.mode == kDone) return draw_nothing(a, b);
+            if (st.mode == kTiles) {
+                look_tiles_alone(a, row, st, sh);
+                draw_from_tiles(a, row, st, b, sh);
+                return;
+            }
+        }
+        __syncthreads();
+    }
+    row_by_bins<T>(a, b, sizeof(T) == 4, sh);
 }
 
 }  // namespace
@@ -745,7 +979,7 @@ extern "C" int hmx_sample_logits(const void* logits, int64_t ld, int64_t B, int6
     if (B == 0 || draws == 0) return HMX_OK;
     if (!logits || !u || !ids || !probs) return HMX_EINVAL;
     SampleArgs a = {logits, ld, (uint32_t)V, u, u_f64 != 0, (int)draws, temperature, top_p, min_p, top_k, temperature_all,
-                    top_p_all, min_p_all, top_k_all, ids, probs, (uint32_t)(hmx_ceil_div(V, (int64_t)kTiles * 256) * 256)};
+                    top_p_all, min_p_all, top_k_all, ids, probs, (uint32_t)(hmx_ceil_div(V, (int64_t)kBins * kTile) * kTile)};
     if (bf16)
         hipLaunchKernelGGL(sample_row_kernel<__bf16>, dim3((unsigned)B), dim3(kThreads), 0, (hipStream_t)stream, a);
     else
