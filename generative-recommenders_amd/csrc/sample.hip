@@ -251,14 +251,16 @@ struct Shared {
         float group[kBins];
     };
     uint32_t ties[kBins];
+    float queue[kWaves * 128];
     State st;
-    u64 wsum[kWaves];
+    u64 wsum[kWaves], wsums[4][kWaves];
     float wmax[kWaves];
-    u64 rest, above, target, total, in_bin;
+    u64 above, in_bin;
     uint32_t bin, n_list, at;
 };
 
-__device__ __forceinline__ void make_table(Shared& sh) {
+template <typename SH>
+__device__ __forceinline__ void make_table(SH& sh) {
     // 2^(i / 128) from the powers that i's bits stand for: a few roundings, and little code
     const double root[7] = {1.0054299011128027, 1.0108892860517005, 1.0218971486541166, 1.0442737824274138,
                             1.0905077326652577, 1.189207115002721, 1.4142135623730951};
@@ -278,6 +280,20 @@ __device__ __forceinline__ u64 block_incl(u64 v, Shared& sh, u64* total) {
     const u64 sums = row_incl(sh.wsum[threadIdx.x & 15]);            // kWaves = 16: one row of lanes
     *total = lane64(sums, 15);
     return v + (wave ? lane64(sums, wave - 1) : 0);
+}
+// The block's sums of N values, in every thread.
+template <int N>
+__device__ __forceinline__ void block_sums(u64 (&v)[N], Shared& sh) {
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        v[q] = wave_incl(v[q]);
+        if ((threadIdx.x & 63) == 63) sh.wsums[q][wave] = v[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] = lane64(row_incl(sh.wsums[q][threadIdx.x & 15]), 15);
 }
 __device__ __forceinline__ float block_max(float v, Shared& sh) {
     for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
@@ -459,8 +475,8 @@ __device__ __forceinline__ void look_gather(const T* row, uint32_t lo, uint32_t 
 }
 
 // Masses by bins of l in sh.bins, which the caller has cleared; returns the thread's sum of all its weights.
-template <typename T>
-__device__ __forceinline__ u64 look_bins(const T* row, uint32_t lo, uint32_t hi, const Row& r, Shared& sh) {
+template <typename T, typename SH>
+__device__ __forceinline__ u64 look_bins(const T* row, uint32_t lo, uint32_t hi, const Row& r, SH& sh) {
     u64 sum = 0;
     each_element<4>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
         u64 w[4];
@@ -494,63 +510,92 @@ __device__ __forceinline__ void look_ranges(const T* row, uint32_t V, const Row&
     __syncthreads();
 }
 
-// bfloat16 values with a counter, in descending order of the value: their place, and the value of a place.
-__device__ __forceinline__ uint32_t place_of_value(uint32_t d, int32_t sign) { return d ^ (uint32_t)(2047 - sign); }      // sign 0 or -1
+// bfloat16 values with a counter have a place in descending order; the value of a place.
 __device__ __forceinline__ float value_of_place(uint32_t place) {
     const uint32_t d = place < 2048 ? 2047 - place : place - 2048;
     return __uint_as_float(((d + kFirstMag) << 16) | (place < 2048 ? 0u : 0x80000000u));
 }
-// Counts by value in sh.count, which the caller has cleared; candidates without a counter go to the list.
-__device__ __forceinline__ void look_values(const __bf16* row, uint32_t lo, uint32_t hi, Shared& sh) {
+// Counts by value in sh.count, which the caller has cleared; candidates without a counter go to the list.  The counters lie
+// by magnitude, the negative ones behind: eight instructions an element, taken from the 16-bit halves as they are.
+__device__ __forceinline__ uint32_t place_of_counter(uint32_t c) { return c < 2048 ? 2047 - c : c; }       // in descending order
+template <typename SH>
+__device__ __forceinline__ void look_values(const __bf16* row, uint32_t lo, uint32_t hi, SH& sh) {
     each_element<8>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t i) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t u = __float_as_uint(l[e]), d = ((u >> 16) & 0x7fffu) - kFirstMag;
-            if (d < 2048) atomicAdd(&sh.count[place_of_value(d, (int32_t)u >> 31)], 1u);
-            else if (candidate(l[e])) append(entry(key_of(l[e]), i + e), sh.list, &sh.n_list);
+            const uint32_t u = __float_as_uint(l[e]), t = (u >> 16) - kFirstMag;      // sign in bit 15, 0 .. 2047 below it
+            if (!(t & 0x7800u)) {
+                const uint32_t at = (t & 0x7ffu) | ((t >> 4) & 0x800u);
+                atomicAdd(&sh.count[at], 1u);
+            } else if (candidate(l[e])) {
+                append(entry(key_of(l[e]), i + e), sh.list, &sh.n_list);
+            }
         }
     });
 }
 
-// Tile by tile of [t0, t1): the weights above khi that pass min_p, and of the elements from klo to khi the count (TIES) or
-// the entries in the list.
+// Tile by tile of [t0, t1): the weights above khi, and of the elements from klo to khi the count (TIES) or the entries in the
+// list.  Values are compared, not keys: two comparisons an element.  Where few are kept, a wave lines them up in its
+// part of `queue` (128 entries) and takes their weights 64 at a time.
 template <typename T>
 __device__ __forceinline__ void look_tiles(const SampleArgs& a, const T* row, const State& st, uint32_t t0, uint32_t t1, const double* tab,
-                                           u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
+                                           float* queue, u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Row r = st.r;
-    const uint32_t klo = st.klo, khi = st.khi;
     const bool count = st.ties;
+    const float above = st.khi < kLowestKey ? -__builtin_inff() : value_of(st.khi);
+    const float from = st.klo <= st.khi ? value_of(st.klo) : __builtin_inff();      // with no border: nothing from `from` to `above`
+    float* line = queue + 128 * wave;
     for (uint32_t t = t0 + wave; t < t1; t += kWaves) {
         u64 w = 0;
-        uint32_t n = 0;
+        uint32_t n = 0, queued = 0;
+        auto flush = [&](uint32_t m) {                               // the first m (at most 64) of the line
+            const u64 x = weight(r, lane < m ? line[lane] : -__builtin_inff(), tab);
+            w += x;
+        };
         each_element<4>(row, t * a.tile, std::min(a.V, (t + 1) * a.tile), lane, 64, [&](const float(&l)[4], uint32_t i) {
-            bool kept[4];
-            bool any = false;
+            u64 kept[4], border[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t key = key_of(l[e]);
-                const bool in = candidate(l[e]) && key >= klo;
-                kept[e] = in && key > khi;
-                any |= kept[e];
-                if (in && !kept[e]) {
-                    if (count) ++n;
-                    else append(entry(key, i + e), list, n_list);
-                }
+                kept[e] = __ballot(l[e] > above);
+                border[e] = __ballot(l[e] >= from) & ~kept[e];
             }
-            if (any) {
+            if (border[0] | border[1] | border[2] | border[3]) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const u64 x = weight(r, l[e], tab);
-                    w += kept[e] && passes(r, l[e]) ? x : 0;
+                    if (count) n += __popcll(border[e]);
+                    else if ((border[e] >> lane) & 1) append(entry(key_of(l[e]), i + e), list, n_list);
                 }
             }
+            if (!(kept[0] | kept[1] | kept[2] | kept[3])) return;
+            if (__popcll(kept[0]) + __popcll(kept[1]) + __popcll(kept[2]) + __popcll(kept[3]) > 64) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w += weight(r, l[e] > above ? l[e] : -__builtin_inff(), tab);
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (l[e] > above) line[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(kept[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)kept[e], 0))] = l[e];
+                queued += __popcll(kept[e]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (queued >= 64) {
+                const float rest = line[64 + lane];
+                flush(64);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                line[lane] = rest;
+                queued -= 64;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
         });
+        if (queued) flush(queued);
         w = wave_incl(w);
-        if (lane == 63) tile[t] = w;
-        if (count) {
-            const u64 c = wave_incl(n);
-            if (lane == 63) ties[t] = (uint32_t)c;
+        if (lane == 63) {
+            tile[t] = w;
+            if (count) ties[t] = n;
         }
     }
 }
@@ -578,6 +623,22 @@ __device__ __forceinline__ void keys_of_bin(const Row& r, int bin, uint32_t* fir
     }
     *last = end[0];
     *first = end[1] + 1;
+}
+
+// Where min_p cuts off the border itself, it is the border: all that passes lies above, nothing apart.
+__device__ __forceinline__ void fold_min_p(State& st) {
+    if (!(st.r.log_min_p > -__builtin_inf())) return;
+    uint32_t lo = kLowestKey - 1, hi = st.r.top;                     // the largest key that does not pass; the maximum does
+#pragma unroll 1
+    while (hi - lo > 1) {
+        const uint32_t step = (hi - lo - 1) / 64 + 1;
+        const u64 at = (u64)lo + (u64)step * ((threadIdx.x & 63) + 1);
+        const int n = __popcll(__ballot(at < hi && !passes(st.r, value_of((uint32_t)at))));
+        const u64 next = (u64)lo + (u64)step * (n + 1);
+        lo += step * n;
+        hi = next < hi ? (uint32_t)next : hi;
+    }
+    if (lo >= st.khi) st.klo = lo + 1, st.khi = lo, st.ties = 1, st.need = 0;
 }
 
 // The lowest key that the gather needs: of the bin in which the k-th largest of the groups' maxima lies (0: below the bins).
@@ -623,13 +684,12 @@ __device__ __forceinline__ void narrow(const SampleArgs& a, const T* row, const 
     }
 }
 
-// sh.bins holds the masses by bins, sh.rest what lies lower: the border of top_p (of the mass `of`; 0: all) for look_tiles.
+// sh.bins holds the masses by bins: the border of top_p of the mass `of` for look_tiles.
 __device__ __forceinline__ void border_by_bins(State& st, u64 of, Shared& sh) {
-    u64 v[kPer], all, sum = 0;
+    u64 v[kPer];
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) v[q] = sh.bins[kPer * threadIdx.x + q], sum += v[q];
-    block_incl(sum, sh, &all);
-    const u64 target = share_of(st.r.p, of ? of : all + sh.rest);
+    for (int q = 0; q < kPer; ++q) v[q] = sh.bins[kPer * threadIdx.x + q];
+    const u64 target = share_of(st.r.p, of);
     find_place(v, target, 0, sh);
     st.need = target - sh.above;
     keys_of_bin(st.r, sh.bin, &st.klo, &st.khi);
@@ -644,7 +704,7 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
     float top = -__builtin_inff(), l[kPer];
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-        c[q] = sh.count[kPer * threadIdx.x + q];
+        c[q] = sh.count[place_of_counter(kPer * threadIdx.x + q)];
         l[q] = value_of_place(kPer * threadIdx.x + q);
         top = c[q] ? fmaxf(top, l[q]) : top;
     }
@@ -676,9 +736,9 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
     u64 of = 0;
 #pragma unroll 1
     for (int pass = r.k > 0 ? 0 : 1; pass < (r.p < 1.0 ? 2 : 1); ++pass) {           // by count, then by mass
-        u64 v[kPer], zone[3] = {0, 0, 0}, sum = 0, all;
+        u64 v[kPer], zone[4] = {0, 0, 0, 0};                         // the list's three, and the counters
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) v[q] = pass ? w[q] * c[q] : c[q], sum += v[q];
+        for (int q = 0; q < kPer; ++q) v[q] = pass ? w[q] * c[q] : c[q], zone[3] += v[q];
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
             const float x = entry_value(sh.list[i]);
             const u64 one = pass ? weight(r, x, sh.tab) : 1;
@@ -687,10 +747,8 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
             zone[1] += at == 1 ? one : 0;
             zone[2] += at == 2 ? one : 0;
         }
-        block_incl(sum, sh, &all);
-#pragma unroll
-        for (int q = 0; q < 3; ++q) block_incl(zone[q], sh, &zone[q]);
-        const u64 total = all + zone[0] + zone[1] + zone[2];
+        block_sums(zone, sh);
+        const u64 total = zone[0] + zone[1] + zone[2] + zone[3];
         if (pass == 0 && (u64)r.k >= total) continue;
         const u64 target = pass ? share_of(r.p, of ? of : total) : (u64)r.k;
         uint32_t place = kBins;
@@ -732,53 +790,45 @@ __device__ __forceinline__ bool draw_from_tiles(const SampleArgs& a, const T* ro
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Row r = st.r;
     const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
-    uint32_t last_key = 0, last_idx = 0;                             // kept are the keys above, and that key up to the index
+    u64 last = (u64)(st.khi + 1) << 32;                              // kept are the entries from it on
     __syncthreads();
-    if (st.ties && st.need) {
-        u64 v[kPer];
+    if (st.need) {
+        if (st.ties) {
+            u64 v[kPer];
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) {
-            const uint32_t t = kPer * threadIdx.x + q;
-            v[q] = t < tiles ? sh.ties[t] : 0;
-        }
-        find_place(v, st.need, 0, sh);
-        const uint32_t t = sh.bin;                                   // the tile of the last kept
-        const float l = value_of(st.khi);
-        const u64 one = passes(r, l) ? weight(r, l, sh.tab) : 0;
-        uint32_t left = (uint32_t)(st.need - sh.above);
-        for (uint32_t i = threadIdx.x; i <= t && i < tiles; i += kThreads) sh.tile[i] += one * (i < t ? sh.ties[i] : left);
-        if (wave == 0) {
-            const uint32_t end = std::min(a.V, (t + 1) * a.tile);
-            for (uint32_t i0 = t * a.tile; i0 < end; i0 += 64) {
-                const uint32_t i = i0 + lane;
+            for (int q = 0; q < kPer; ++q) {
+                const uint32_t t = kPer * threadIdx.x + q;
+                v[q] = t < tiles ? sh.ties[t] : 0;
+            }
+            find_place(v, st.need, 0, sh);
+            const uint32_t t = sh.bin, end = std::min(a.V, (t + 1) * a.tile);        // the tile of the last kept
+            const uint32_t left = (uint32_t)(st.need - sh.above);
+            const u64 one = weight(r, value_of(st.khi), sh.tab);
+            for (uint32_t i = threadIdx.x; i <= t && i < tiles; i += kThreads) sh.tile[i] += one * (i < t ? sh.ties[i] : left);
+            u64 carry = 0, all;
+            for (uint32_t i0 = t * a.tile; i0 < end; i0 += kThreads) {
+                const uint32_t i = i0 + threadIdx.x;
                 const float x = i < end ? (float)row[i] : __builtin_nanf("");
                 const bool tie = candidate(x) && key_of(x) == st.khi;
-                const u64 all = __ballot(tie);
-                const uint32_t here = __popcll(all);
-                if (here < left) {
-                    left -= here;
-                    continue;
-                }
-                if (tie && __popcll(all & ((1ull << lane) - 1)) == left - 1) sh.at = i;
-                break;
+                const u64 upto = carry + block_incl(tie, sh, &all);
+                if (tie && upto == left) sh.at = i;
+                carry += all;
             }
+            __syncthreads();
+            last = entry(st.khi, sh.at);
+        } else {
+            const uint32_t n = sh.n_list;
+            if (n > kBins) return false;
+            sort_list<true>(n, sh.list);
+            const uint32_t place = place_of_mass(r, n, st.need, sh);
+            for (uint32_t i = threadIdx.x; i <= place; i += kThreads) {
+                const u64 y = sh.list[i];
+                const float l = entry_value(y);
+                if (passes(r, l)) atomicAdd(&sh.tile[~(uint32_t)y / a.tile], weight(r, l, sh.tab));
+            }
+            last = sh.list[place];
+            __syncthreads();
         }
-        __syncthreads();
-        last_key = st.khi;
-        last_idx = sh.at;
-    } else if (!st.ties) {
-        const uint32_t n = sh.n_list;
-        if (n > kBins) return false;
-        sort_list<true>(n, sh.list);
-        const uint32_t last = place_of_mass(r, n, st.need, sh);
-        for (uint32_t i = threadIdx.x; i <= last; i += kThreads) {
-            const u64 y = sh.list[i];
-            const float l = entry_value(y);
-            if (passes(r, l)) atomicAdd(&sh.tile[~(uint32_t)y / a.tile], weight(r, l, sh.tab));
-        }
-        last_key = (uint32_t)(sh.list[last] >> 32);
-        last_idx = ~(uint32_t)sh.list[last];
-        __syncthreads();
     }
     u64 w[kPer], sum = 0, total;
 #pragma unroll
@@ -806,8 +856,7 @@ __device__ __forceinline__ bool draw_from_tiles(const SampleArgs& a, const T* ro
             u64 x[4], four = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t key = key_of(l[e]);
-                const bool kept = candidate(l[e]) && (key > last_key || (key == last_key && i + e <= last_idx)) && passes(r, l[e]);
+                const bool kept = candidate(l[e]) && entry(key_of(l[e]), i + e) >= last && passes(r, l[e]);
                 const u64 one = weight(r, l[e], sh.tab);
                 x[e] = kept ? one : 0;
                 four += x[e];
@@ -842,7 +891,7 @@ __device__ __forceinline__ void look_tiles_alone(const SampleArgs& a, const T* r
     __syncthreads();
     if (threadIdx.x == 0) sh.n_list = 0;
     __syncthreads();
-    look_tiles(a, row, st, 0, (a.V + a.tile - 1) / a.tile, sh.tab, sh.tile, sh.ties, sh.list, &sh.n_list);
+    look_tiles(a, row, st, 0, (a.V + a.tile - 1) / a.tile, sh.tab, sh.queue, sh.tile, sh.ties, sh.list, &sh.n_list);
     __syncthreads();
 }
 
@@ -907,20 +956,17 @@ __device__ __forceinline__ void row_by_bins(const SampleArgs& a, int64_t b, bool
         __syncthreads();
         for (int q = 0; q < kPer; ++q) sh.bins[q * kThreads + threadIdx.x] = 0;
         __syncthreads();
-        const u64 mine = look_bins(row, 0, a.V, r, sh);
-        u64 all, in_bins, sum = 0;
-        block_incl(mine, sh, &all);
-        for (int q = 0; q < kPer; ++q) sum += sh.bins[q * kThreads + threadIdx.x];
-        block_incl(sum, sh, &in_bins);
-        if (threadIdx.x == 0) sh.rest = all - in_bins;
-        __syncthreads();
-        border_by_bins(st, of, sh);
+        u64 sum[1] = {look_bins(row, 0, a.V, r, sh)};
+        block_sums(sum, sh);
+        border_by_bins(st, of ? of : sum[0], sh);
+        fold_min_p(st);
         look_tiles_alone(a, row, st, sh);
         if (draw_from_tiles(a, row, st, b, sh)) return;
         narrow<T, true>(a, row, r, st.klo, &st.khi, &st.need, sh);
         st.klo = st.khi;
         st.ties = 1;
     }
+    fold_min_p(st);
     look_tiles_alone(a, row, st, sh);
     draw_from_tiles(a, row, st, b, sh);
 }
@@ -956,6 +1002,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
             border_by_values(a, st, sh.n_list, sh);
             if (st.mode == kDone) return draw_nothing(a, b);
             if (st.mode == kTiles) {
+                fold_min_p(st);
                 look_tiles_alone(a, row, st, sh);
                 draw_from_tiles(a, row, st, b, sh);
                 return;
@@ -966,24 +1013,276 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     row_by_bins<T>(a, b, sizeof(T) == 4, sh);
 }
 
+// ------------------------------------------------------------------------------- many blocks, one row
+// Between the kernels a row's state lies in the workspace.  The looks run on gridDim.x segments of whole tiles a row, the
+// steps between them on one block a row.
+struct RowSpace {
+    u64 bins[kBins];                // the first half of it: counts of bfloat16 values
+    u64 tile[kBins];
+    u64 list[kBins];
+    uint32_t ties[kBins];
+    float group[kBins];
+    u64 mass;
+    State st;
+    uint32_t n_list;
+};
+
+struct Segment {
+    uint32_t t0, t1, lo, hi;        // tiles and elements
+};
+__device__ __forceinline__ Segment segment(const SampleArgs& a) {
+    const uint32_t tiles = (a.V + a.tile - 1) / a.tile, per = (tiles + gridDim.x - 1) / gridDim.x;
+    Segment s;
+    s.t0 = std::min(blockIdx.x * per, tiles);
+    s.t1 = std::min(s.t0 + per, tiles);
+    s.lo = s.t0 * a.tile;
+    s.hi = std::min(a.V, s.t1 * a.tile);
+    return s;
+}
+
+// fp32: the maxima of the 64 groups of each segment; clears what later kernels add to.
+template <typename T>
+__global__ __launch_bounds__(kThreads, 8) void split_max_kernel(SampleArgs a, RowSpace* ws) {
+    RowSpace& w = ws[blockIdx.y];
+    const Segment s = segment(a);
+    for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < kBins; i += gridDim.x * kThreads) w.bins[i] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) w.n_list = 0, w.mass = 0;
+    float top = s.t0 < s.t1 ? look_max((const T*)a.logits + blockIdx.y * a.ld, s.lo, s.hi) : -__builtin_inff();
+    for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if ((threadIdx.x & 15) == 0) w.group[blockIdx.x * 64 + threadIdx.x / 16] = top;
+}
+
+__global__ __launch_bounds__(kThreads) void split_clear_kernel(RowSpace* ws) {
+    RowSpace& w = ws[blockIdx.x];
+    for (int i = threadIdx.x; i < kBins / 2; i += kThreads) w.bins[i] = 0;
+    if (threadIdx.x == 0) w.n_list = 0;
+}
+
+// bfloat16: the counts of the values.
+struct SharedValues {
+    uint32_t count[kBins];
+    u64 list[kBins];
+    uint32_t n_list, base;
+};
+__global__ __launch_bounds__(kThreads, 8) void split_values_kernel(SampleArgs a, RowSpace* ws) {
+    __shared__ SharedValues sh;
+    RowSpace& w = ws[blockIdx.y];
+    const Segment s = segment(a);
+    for (int q = 0; q < kPer; ++q) sh.count[q * kThreads + threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.n_list = 0;
+    __syncthreads();
+    if (s.t0 < s.t1) look_values((const __bf16*)a.logits + blockIdx.y * a.ld, s.lo, s.hi, sh);
+    __syncthreads();
+    uint32_t* count = reinterpret_cast<uint32_t*>(w.bins);
+    for (int q = 0; q < kPer; ++q) {
+        const uint32_t c = sh.count[q * kThreads + threadIdx.x];
+        if (c) atomicAdd(&count[q * kThreads + threadIdx.x], c);
+    }
+    if (threadIdx.x == 0) sh.base = sh.n_list ? atomicAdd(&w.n_list, sh.n_list) : 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < sh.n_list && i < kBins; i += kThreads)
+        if (sh.base + i < kBins) w.list[sh.base + i] = sh.list[i];
+}
+
+// What the looks have to do, from the groups' maxima (fp32) or the counts (bfloat16).
+template <typename T>
+__global__ __launch_bounds__(kThreads) void split_plan_kernel(SampleArgs a, RowSpace* ws, int groups) {
+    __shared__ Shared sh;
+    const int64_t b = blockIdx.x;
+    RowSpace& w = ws[b];
+    make_table(sh);
+    State st;
+    st.r = settings(a, b);
+    st.mode = kAlone;
+    st.klo = 1, st.khi = 0;
+    st.ties = 1;
+    st.need = 0;
+    Row& r = st.r;
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t n = w.n_list;
+        if (n <= kBins) {
+            const uint32_t* count = reinterpret_cast<const uint32_t*>(w.bins);
+            for (int q = 0; q < kPer; ++q) sh.count[q * kThreads + threadIdx.x] = count[q * kThreads + threadIdx.x];
+            for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.list[i] = w.list[i];
+            __syncthreads();
+            border_by_values(a, st, n, sh);
+        }
+    } else {
+        float top = -__builtin_inff();
+        for (int g = threadIdx.x; g < groups; g += kThreads) {
+            sh.group[g] = w.group[g];
+            top = fmaxf(top, sh.group[g]);
+        }
+        top = block_max(top, sh);
+        if (!candidate(top)) {
+            st.mode = kDone;
+        } else if (by_maxima(r, groups)) {
+            set_scale(r, top, (float)kBins);
+            set_bins(r, kRange);
+            st.klo = key_by_maxima(r, groups, sh);
+            st.mode = st.klo ? kGather : kAlone;
+        } else if (r.k == 0) {
+            const float by = (float)(1.4426950408889634 * r.inv_t);
+            float least = 0.f;
+            for (int g = threadIdx.x; g < groups; g += kThreads) {
+                const float m = sh.group[g];
+                least += m == top ? 1.f : candidate(m) ? __builtin_amdgcn_exp2f((m - top) * by) : 0.f;
+            }
+            least = 0.99f * block_sum(least, sh);
+            const uint32_t tiles = (a.V + a.tile - 1) / a.tile, per = (tiles + groups / 64 - 1) / (groups / 64);
+            set_scale(r, top, 1.03f * least * (float)per * (float)(a.tile / 64 + 64));       // elements of a group at most
+            if (r.p < 1.0) {
+                set_bins(r, range_for(r, a.V, least));
+                st.mode = kBinning;
+            } else {
+                st.mode = kTiles;
+            }
+        }
+    }
+    if (st.mode == kDone) draw_nothing(a, b);
+    if (st.mode == kTiles) fold_min_p(st);
+    if (threadIdx.x == 0) w.st = st;
+}
+
+struct SharedLook {
+    double tab[128];
+    u64 bins[kBins];
+    float queue[kWaves * 128];
+    u64 mass;
+};
+template <typename T>
+__global__ __launch_bounds__(kThreads, 8) void split_look_kernel(SampleArgs a, RowSpace* ws) {
+    __shared__ SharedLook sh;
+    RowSpace& w = ws[blockIdx.y];
+    const T* row = (const T*)a.logits + blockIdx.y * a.ld;
+    const int mode = w.st.mode;
+    if (mode == kDone || mode == kAlone) return;
+    const Segment s = segment(a);
+    if (s.t0 >= s.t1) return;
+    make_table(sh);
+    if (mode == kTiles) {
+        __syncthreads();
+        look_tiles(a, row, w.st, s.t0, s.t1, sh.tab, sh.queue, w.tile, w.ties, w.list, &w.n_list);
+        return;
+    }
+    if (mode == kGather) {
+        look_gather(row, s.lo, s.hi, w.st.klo, w.list, &w.n_list);
+        return;
+    }
+    for (int q = 0; q < kPer; ++q) sh.bins[q * kThreads + threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.mass = 0;
+    __syncthreads();
+    const u64 mine = wave_incl(look_bins(row, s.lo, s.hi, w.st.r, sh));
+    if ((threadIdx.x & 63) == 63) atomicAdd(&sh.mass, mine);
+    __syncthreads();
+    for (int q = 0; q < kPer; ++q) {
+        const u64 m = sh.bins[q * kThreads + threadIdx.x];
+        if (m) atomicAdd(&w.bins[q * kThreads + threadIdx.x], m);
+    }
+    if (threadIdx.x == 0) atomicAdd(&w.mass, sh.mass);
+}
+
+// After a look: the draws, or (bins) the border and what the next look has to do.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void split_border_kernel(SampleArgs a, RowSpace* ws) {
+    __shared__ Shared sh;
+    const int64_t b = blockIdx.x;
+    RowSpace& w = ws[b];
+    const T* row = (const T*)a.logits + b * a.ld;
+    const int mode = w.st.mode;
+    if (mode == kDone) return;
+    make_table(sh);
+    bool alone = mode == kAlone;
+    if (mode == kGather) {
+        const uint32_t n = w.n_list;
+        if (n <= kBins) {
+            for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.list[i] = w.list[i];
+            __syncthreads();
+            draw_from_list(a, w.st.r, b, n, sh);
+        } else {
+            alone = true;
+        }
+    } else if (mode == kBinning) {
+        for (int q = 0; q < kPer; ++q) sh.bins[q * kThreads + threadIdx.x] = w.bins[q * kThreads + threadIdx.x];
+        __syncthreads();
+        State st = w.st;
+        border_by_bins(st, w.mass, sh);
+        fold_min_p(st);
+        __syncthreads();
+        if (threadIdx.x == 0) w.st = st, w.n_list = 0;
+        return;
+    } else if (mode == kTiles) {
+        const State st = w.st;
+        for (int q = 0; q < kPer; ++q) {
+            const int t = q * kThreads + threadIdx.x;
+            sh.tile[t] = w.tile[t];
+            if (st.ties) sh.ties[t] = w.ties[t];
+        }
+        const uint32_t n = st.ties ? 0 : w.n_list;
+        if (threadIdx.x == 0) sh.n_list = n;
+        for (uint32_t i = threadIdx.x; i < n && i < kBins; i += kThreads) sh.list[i] = w.list[i];
+        __syncthreads();
+        alone = !draw_from_tiles(a, row, st, b, sh);
+    }
+    __syncthreads();
+    if (alone) row_by_bins<T>(a, b, false, sh);
+    if (threadIdx.x == 0) w.st.mode = kDone;
+}
+
+// Blocks over which a row is cut: enough to have two on each of the card's 256 compute units, segments of 4096 elements
+// (one step of a block) at least; 1: not cut.
+int splits(int64_t B, int64_t V) {
+    const int64_t c = std::min<int64_t>(std::min<int64_t>(512 / B, V / 4096), kMaxSplit);
+    return V > kSmall && c >= 2 ? (int)c : 1;
+}
+
+template <typename T>
+void launch_split(const SampleArgs& a, int64_t B, int C, RowSpace* ws, hipStream_t st) {
+    const dim3 wide((unsigned)C, (unsigned)B), one((unsigned)B), block(kThreads);
+    if constexpr (sizeof(T) == 2) {
+        hipLaunchKernelGGL(split_clear_kernel, one, block, 0, st, ws);
+        hipLaunchKernelGGL(split_values_kernel, wide, block, 0, st, a, ws);
+    } else {
+        hipLaunchKernelGGL(split_max_kernel<T>, wide, block, 0, st, a, ws);
+    }
+    hipLaunchKernelGGL(split_plan_kernel<T>, one, block, 0, st, a, ws, 64 * C);
+    hipLaunchKernelGGL(split_look_kernel<T>, wide, block, 0, st, a, ws);
+    hipLaunchKernelGGL(split_border_kernel<T>, one, block, 0, st, a, ws);
+    // rows that top_p may send over bins have one more look
+    if (sizeof(T) == 4 && (a.top_p || a.p < 1.0)) {
+        hipLaunchKernelGGL(split_look_kernel<T>, wide, block, 0, st, a, ws);
+        hipLaunchKernelGGL(split_border_kernel<T>, one, block, 0, st, a, ws);
+    }
+}
+
 }  // namespace
 
 // ================================================================================ C ABI
+extern "C" size_t hmx_sample_logits_workspace_bytes(int64_t B, int64_t V) {
+    return B > 0 && V > 0 && splits(B, V) > 1 ? (size_t)B * sizeof(RowSpace) : 0;
+}
+
 extern "C" int hmx_sample_logits(const void* logits, int64_t ld, int64_t B, int64_t V, int bf16, const void* u, int u_f64,
                                  int64_t draws, const float* temperature, const int32_t* top_k, const float* top_p,
                                  const float* min_p, double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all,
-                                 int64_t* ids, float* probs, void* stream) {
+                                 int64_t* ids, float* probs, void* workspace, size_t workspace_bytes, void* stream) {
     HMX_ENTER();
     if (B < 0 || V < 1 || V >= (int64_t)1 << 31 || draws < 0 || draws >= (int64_t)1 << 31 || ld < 0 || B >= (int64_t)1 << 22)
         return HMX_EINVAL;
     if (B == 0 || draws == 0) return HMX_OK;
     if (!logits || !u || !ids || !probs) return HMX_EINVAL;
+    const int C = splits(B, V);
+    if (workspace_bytes < hmx_sample_logits_workspace_bytes(B, V) || (C > 1 && !workspace)) return HMX_EWORKSPACE;
     SampleArgs a = {logits, ld, (uint32_t)V, u, u_f64 != 0, (int)draws, temperature, top_p, min_p, top_k, temperature_all,
                     top_p_all, min_p_all, top_k_all, ids, probs, (uint32_t)(hmx_ceil_div(V, (int64_t)kBins * kTile) * kTile)};
-    if (bf16)
+    if (C > 1) {
+        if (bf16) launch_split<__bf16>(a, B, C, (RowSpace*)workspace, (hipStream_t)stream);
+        else launch_split<float>(a, B, C, (RowSpace*)workspace, (hipStream_t)stream);
+    } else if (bf16) {
         hipLaunchKernelGGL(sample_row_kernel<__bf16>, dim3((unsigned)B), dim3(kThreads), 0, (hipStream_t)stream, a);
-    else
+    } else {
         hipLaunchKernelGGL(sample_row_kernel<float>, dim3((unsigned)B), dim3(kThreads), 0, (hipStream_t)stream, a);
+    }
     HMX_CHECK_LAUNCH();
     return HMX_OK;
 }

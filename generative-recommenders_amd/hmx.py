@@ -160,7 +160,8 @@ PROTOTYPES = {
     "hmx_mx_dequantize": (c_int, [P, P, I64, I64, c_int, c_int, P, P]),
     "hmx_linear_mx4": (c_int, [P, I64, P, c_int, I64, P, P, I64, I64, c_int, P, P]),
     "hmx_sample_logits": (c_int, [P, I64, I64, I64, c_int, P, c_int, I64, P, P, P, P, ctypes.c_double, I64, ctypes.c_double,
-                                  ctypes.c_double, P, P, P]),
+                                  ctypes.c_double, P, P, P, c_size_t, P]),
+    "hmx_sample_logits_workspace_bytes": (c_size_t, [I64, I64]),
     "hmx_profile_enable": (c_int, [c_int]),
     "hmx_profile_filter": (c_int, [c_char_p]),
     "hmx_profile_collect": (c_int, [c_char_p, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(c_int64)]),

@@ -698,10 +698,11 @@ int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, int x_kind,
  * below 1.  temperature, top_k, top_p, min_p (B) or NULL: then the numbers behind them hold for every row.  Sums are
  * integers of a fixed unit per row (at most 2^-51 of the largest weight where the row's mass is below 2^11), so results
  * do not depend on the order of any addition.  V < 2^31, B < 2^22. */
+size_t hmx_sample_logits_workspace_bytes(int64_t B, int64_t V);
 int hmx_sample_logits(const void* logits, int64_t ld, int64_t B, int64_t V, int bf16, const void* u, int u_f64, int64_t draws,
                       const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                       double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all, int64_t* ids, float* probs,
-                      void* stream);
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -57,9 +57,13 @@ def test_python_entries_refuse_cpu_tensors():
 def test_sample_entry():
     L = hmx.lib()
     good = dict(logits=P, ld=64, B=4, V=64, bf16=0, u=P, u64=0, draws=1, t=None, k=None, p=None, mp=None, ta=1.0, ka=0, pa=1.0,
-                mpa=0.0, ids=P, probs=P, stream=None)
+                mpa=0.0, ids=P, probs=P, ws=None, ws_bytes=0, stream=None)
     for bad in (dict(logits=None), dict(ld=-1), dict(B=-1), dict(V=0), dict(V=1 << 31), dict(u=None), dict(draws=-1),
                 dict(ids=None), dict(probs=None), dict(B=1 << 22)):
         assert L.hmx_sample_logits(*{**good, **bad}.values()) == EINVAL, bad
+    nbytes = L.hmx_sample_logits_workspace_bytes(4, 1 << 20)
+    assert nbytes > 0 and L.hmx_sample_logits_workspace_bytes(4, 64) == 0
+    for bad in (dict(ws=P, ws_bytes=nbytes - 1), dict(ws=None, ws_bytes=nbytes)):
+        assert L.hmx_sample_logits(*{**good, "V": 1 << 20, "ld": 1 << 20, **bad}.values()) == -2
     assert L.hmx_sample_logits(*{**good, "B": 0, "logits": None}.values()) == 0
     assert L.hmx_sample_logits(*{**good, "draws": 0}.values()) == 0
