@@ -200,7 +200,7 @@ __device__ __forceinline__ float range_for(const Row& r, uint32_t V, float least
 }
 // Whether the k-th largest of `groups` maxima leads to a list: groups * ln(groups / (groups - k)) elements reach it where the
 // groups are alike, 1650 of 1024 groups, 2750 of 4096 at most.
-__device__ __forceinline__ bool by_maxima(const Row& r, int groups) { return r.k > 0 && 5 * r.k <= 4 * groups && r.k <= 2000; }
+__host__ __device__ inline bool by_maxima(int64_t k, int groups) { return k > 0 && 5 * k <= 4 * groups && k <= 2000; }
 
 // ------------------------------------------------------------------------------- block sums
 // v of the lane that the DPP control names; 0 where there is none, or where the row mask leaves the lane out.
@@ -243,7 +243,6 @@ struct Shared {
     union {
         u64 bins[kBins];
         uint32_t count[kBins];
-        u64 run[kBins];
         u64 tile[kBins];
     };
     union {
@@ -400,48 +399,108 @@ __device__ __forceinline__ void draw_nothing(const SampleArgs& a, int64_t b) {
     for (int q = threadIdx.x; q < a.draws; q += kThreads) a.ids[b * a.draws + q] = -1, a.probs[b * a.draws + q] = 0.f;
 }
 
-// The draws of a row whose first top_k elements (all, where that is off) are among the list's n entries.
-__device__ __forceinline__ void draw_from_list(const SampleArgs& a, const Row& r, int64_t b, uint32_t n, Shared& sh) {
-    uint32_t keep = n;
-    if ((r.k > 0 && r.k < n) || r.p < 1.0) {
-        sort_list<true>(n, sh.list);
-        if (r.k > 0 && r.k < n) keep = (uint32_t)r.k;
-    }
-    if (r.p < 1.0) {
-        u64 sum = 0, total;
-        for (uint32_t i = threadIdx.x; i < keep; i += kThreads) sum += weight(r, entry_value(sh.list[i]), sh.tab);
-        block_incl(sum, sh, &total);
-        keep = place_of_mass(r, keep, share_of(r.p, total), sh) + 1;
-    }
-    // the kept entries in index order, with their running sums (below min_p: weight zero)
-    for (uint32_t i = threadIdx.x; i < keep; i += kThreads) {
-        const u64 x = sh.list[i];
-        sh.list[i] = ((u64)(~(uint32_t)x) << 32) | (uint32_t)(x >> 32);
-    }
-    sort_list<false>(keep, sh.list);
-    u64 v[kPer], sum = 0, total;
+// The draws by the tiles' sums (sh.tile): the kept elements are the entries from `last` on that pass min_p.  One wave a draw
+// finds the tile by running sums, then the element, 1024 elements' loads at once.
+template <typename T>
+__device__ __forceinline__ void draw_by_tiles(const SampleArgs& a, const T* row, const Row& r, u64 last, int64_t b, Shared& sh) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
+    u64 w[kPer], sum = 0, total;
+    __syncthreads();
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-        const uint32_t i = kPer * threadIdx.x + q;
-        const float l = i < keep ? value_of((uint32_t)sh.list[i]) : -__builtin_inff();
-        v[q] = i < keep && passes(r, l) ? weight(r, l, sh.tab) : 0;
-        sum += v[q];
+        const uint32_t t = kPer * threadIdx.x + q;
+        w[q] = t < tiles ? sh.tile[t] : 0;
+        sum += w[q];
     }
     u64 upto = block_incl(sum, sh, &total) - sum;
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) upto += v[q], sh.run[kPer * threadIdx.x + q] = upto;
+    for (int q = 0; q < kPer; ++q) upto += w[q], sh.tile[kPer * threadIdx.x + q] = upto;
     __syncthreads();
-    for (int q = threadIdx.x; q < a.draws; q += kThreads) {
+    for (int q = wave; q < a.draws; q += kWaves) {
         const u64 want = draw_target(a, b * a.draws + q, total);
-        uint32_t lo = 0, hi = keep - 1;                              // the first with a running sum above `want`
+        uint32_t lo = 0, hi = tiles - 1;
         while (lo < hi) {
             const uint32_t mid = (lo + hi) / 2;
-            if (sh.run[mid] > want) hi = mid;
+            if (sh.tile[mid] > want) hi = mid;
             else lo = mid + 1;
         }
-        const u64 x = sh.list[lo];
-        put_draw(a, r, b * a.draws + q, (uint32_t)(x >> 32), value_of((uint32_t)x), total, sh.tab);
+        u64 before = lo ? sh.tile[lo - 1] : 0;
+        const uint32_t end = std::min(a.V, (lo + 1) * a.tile);
+        bool found = false;
+#pragma unroll 1
+        for (uint32_t i0 = lo * a.tile; i0 < end && !found; i0 += kTile) {
+            float l[4][4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l[g][e] = (float)row[std::min(i0 + 256 * g + 4 * lane + e, a.V - 1)];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (found) continue;
+                u64 x[4], four = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t i = i0 + 256 * g + 4 * lane + e;
+                    const bool kept = i < end && candidate(l[g][e]) && entry(key_of(l[g][e]), i) >= last && passes(r, l[g][e]);
+                    x[e] = kept ? weight(r, l[g][e], sh.tab) : 0;
+                    four += x[e];
+                }
+                const u64 sums = before + wave_incl(four);
+                const u64 hit = __ballot(sums > want);
+                before = lane64(sums, 63);
+                if (hit) {
+                    found = true;
+                    if (lane == __ffsll((long long)hit) - 1) {
+                        u64 at = sums - four;
+                        float l0 = l[g][0];
+                        uint32_t e0 = 0;
+                        bool past = false;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            at += x[e];
+                            if (!past) l0 = l[g][e], e0 = e;
+                            past |= at > want;
+                        }
+                        put_draw(a, r, b * a.draws + q, i0 + 256 * g + 4 * lane + e0, l0, total, sh.tab);
+                    }
+                }
+            }
+        }
     }
+}
+
+// Adds the weights of the list's first n entries that pass min_p to their tiles.
+__device__ __forceinline__ void list_to_tiles(const SampleArgs& a, const Row& r, uint32_t n, Shared& sh) {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        const u64 x = sh.list[i];
+        const float l = entry_value(x);
+        if (passes(r, l)) atomicAdd(&sh.tile[~(uint32_t)x / a.tile], weight(r, l, sh.tab));
+    }
+}
+
+// The draws of a row whose first top_k elements (all, where that is off) are among the list's n entries, which are the
+// row's elements from klo on.
+template <typename T>
+__device__ __forceinline__ void draw_from_list(const SampleArgs& a, const T* row, const Row& r, int64_t b, uint32_t n, uint32_t klo, Shared& sh) {
+    uint32_t keep = n;
+    u64 last = (u64)klo << 32;
+    if ((r.k > 0 && r.k < n) || r.p < 1.0) {
+        sort_list<true>(n, sh.list);
+        if (r.k > 0 && r.k < n) keep = (uint32_t)r.k;
+        if (r.p < 1.0) {
+            u64 total[1] = {0};
+            for (uint32_t i = threadIdx.x; i < keep; i += kThreads) total[0] += weight(r, entry_value(sh.list[i]), sh.tab);
+            block_sums(total, sh);
+            keep = place_of_mass(r, keep, share_of(r.p, total[0]), sh) + 1;
+        }
+        last = sh.list[keep - 1];
+    }
+    __syncthreads();
+    for (int q = 0; q < kPer; ++q) sh.tile[q * kThreads + threadIdx.x] = 0;
+    __syncthreads();
+    list_to_tiles(a, r, keep, sh);
+    draw_by_tiles(a, row, r, last, b, sh);
 }
 
 // ------------------------------------------------------------------------------- looks at the elements
@@ -787,7 +846,6 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
 // draws.  False: the list has overflown.
 template <typename T>
 __device__ __forceinline__ bool draw_from_tiles(const SampleArgs& a, const T* row, const State& st, int64_t b, Shared& sh) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Row r = st.r;
     const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
     u64 last = (u64)(st.khi + 1) << 32;                              // kept are the entries from it on
@@ -821,67 +879,12 @@ __device__ __forceinline__ bool draw_from_tiles(const SampleArgs& a, const T* ro
             if (n > kBins) return false;
             sort_list<true>(n, sh.list);
             const uint32_t place = place_of_mass(r, n, st.need, sh);
-            for (uint32_t i = threadIdx.x; i <= place; i += kThreads) {
-                const u64 y = sh.list[i];
-                const float l = entry_value(y);
-                if (passes(r, l)) atomicAdd(&sh.tile[~(uint32_t)y / a.tile], weight(r, l, sh.tab));
-            }
+            list_to_tiles(a, r, place + 1, sh);
             last = sh.list[place];
             __syncthreads();
         }
     }
-    u64 w[kPer], sum = 0, total;
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        const uint32_t t = kPer * threadIdx.x + q;
-        w[q] = t < tiles ? sh.tile[t] : 0;
-        sum += w[q];
-    }
-    u64 upto = block_incl(sum, sh, &total) - sum;
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) upto += w[q], sh.tile[kPer * threadIdx.x + q] = upto;
-    __syncthreads();
-    for (int q = wave; q < a.draws; q += kWaves) {
-        const u64 want = draw_target(a, b * a.draws + q, total);
-        uint32_t lo = 0, hi = tiles - 1;
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (sh.tile[mid] > want) hi = mid;
-            else lo = mid + 1;
-        }
-        u64 before = lo ? sh.tile[lo - 1] : 0;
-        bool found = false;
-        each_element<4>(row, lo * a.tile, std::min(a.V, (lo + 1) * a.tile), lane, 64, [&](const float(&l)[4], uint32_t i) {
-            if (found) return;
-            u64 x[4], four = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool kept = candidate(l[e]) && entry(key_of(l[e]), i + e) >= last && passes(r, l[e]);
-                const u64 one = weight(r, l[e], sh.tab);
-                x[e] = kept ? one : 0;
-                four += x[e];
-            }
-            const u64 sums = before + wave_incl(four);
-            const u64 hit = __ballot(sums > want);
-            before = lane64(sums, 63);
-            if (hit) {
-                found = true;
-                if (lane == __ffsll((long long)hit) - 1) {
-                    u64 at = sums - four;
-                    float l0 = l[0];
-                    uint32_t e0 = 0;
-                    bool past = false;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        at += x[e];
-                        if (!past) l0 = l[e], e0 = e;
-                        past |= at > want;
-                    }
-                    put_draw(a, r, b * a.draws + q, i + e0, l0, total, sh.tab);
-                }
-            }
-        });
-    }
+    draw_by_tiles(a, row, r, last, b, sh);
     return true;
 }
 
@@ -905,7 +908,7 @@ __device__ __forceinline__ void row_by_bins(const SampleArgs& a, int64_t b, bool
     const float own = look_max(row, 0, a.V);
     const float top = block_max(own, sh);
     if (!candidate(top)) return draw_nothing(a, b);
-    if (quick && by_maxima(r, kThreads)) {
+    if (quick && by_maxima(r.k, kThreads)) {
         set_scale(r, top, (float)kBins);
         set_bins(r, kRange);
         if (threadIdx.x == 0) sh.n_list = 0;
@@ -914,7 +917,7 @@ __device__ __forceinline__ void row_by_bins(const SampleArgs& a, int64_t b, bool
         if (klo) {
             look_gather(row, 0, a.V, klo, sh.list, &sh.n_list);
             __syncthreads();
-            if (sh.n_list <= kBins) return draw_from_list(a, r, b, sh.n_list, sh);
+            if (sh.n_list <= kBins) return draw_from_list(a, row, r, b, sh.n_list, klo, sh);
         }
     }
     // the maxima of the threads bound the mass from below and, as often as a thread has elements, from above
@@ -991,7 +994,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
         if (!candidate(top)) return draw_nothing(a, b);
         Row r = settings(a, b);
         set_scale(r, top, (float)kSmall);
-        return draw_from_list(a, r, b, sh.n_list, sh);
+        return draw_from_list(a, row, r, b, sh.n_list, kLowestKey, sh);
     }
     if constexpr (sizeof(T) == 2) {
         look_values(row, 0, a.V, sh);
@@ -1058,6 +1061,16 @@ __global__ __launch_bounds__(kThreads) void split_clear_kernel(RowSpace* ws) {
     if (threadIdx.x == 0) w.n_list = 0;
 }
 
+// Appends the block's list (which may have overflown) to the row's.
+template <typename SH>
+__device__ __forceinline__ void to_row_list(SH& sh, RowSpace& w) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.base = sh.n_list ? atomicAdd(&w.n_list, sh.n_list) : 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < sh.n_list && i < kBins; i += kThreads)
+        if (sh.base < kBins && i < kBins - sh.base) w.list[sh.base + i] = sh.list[i];
+}
+
 // bfloat16: the counts of the values.
 struct SharedValues {
     uint32_t count[kBins];
@@ -1078,10 +1091,7 @@ __global__ __launch_bounds__(kThreads, 8) void split_values_kernel(SampleArgs a,
         const uint32_t c = sh.count[q * kThreads + threadIdx.x];
         if (c) atomicAdd(&count[q * kThreads + threadIdx.x], c);
     }
-    if (threadIdx.x == 0) sh.base = sh.n_list ? atomicAdd(&w.n_list, sh.n_list) : 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < sh.n_list && i < kBins; i += kThreads)
-        if (sh.base + i < kBins) w.list[sh.base + i] = sh.list[i];
+    to_row_list(sh, w);
 }
 
 // What the looks have to do, from the groups' maxima (fp32) or the counts (bfloat16).
@@ -1116,7 +1126,7 @@ __global__ __launch_bounds__(kThreads) void split_plan_kernel(SampleArgs a, RowS
         top = block_max(top, sh);
         if (!candidate(top)) {
             st.mode = kDone;
-        } else if (by_maxima(r, groups)) {
+        } else if (by_maxima(r.k, groups)) {
             set_scale(r, top, (float)kBins);
             set_bins(r, kRange);
             st.klo = key_by_maxima(r, groups, sh);
@@ -1146,9 +1156,13 @@ __global__ __launch_bounds__(kThreads) void split_plan_kernel(SampleArgs a, RowS
 
 struct SharedLook {
     double tab[128];
-    u64 bins[kBins];
+    union {
+        u64 bins[kBins];
+        u64 list[kBins];
+    };
     float queue[kWaves * 128];
     u64 mass;
+    uint32_t n_list, base;
 };
 template <typename T>
 __global__ __launch_bounds__(kThreads, 8) void split_look_kernel(SampleArgs a, RowSpace* ws) {
@@ -1166,7 +1180,11 @@ __global__ __launch_bounds__(kThreads, 8) void split_look_kernel(SampleArgs a, R
         return;
     }
     if (mode == kGather) {
-        look_gather(row, s.lo, s.hi, w.st.klo, w.list, &w.n_list);
+        // by way of LDS: an atomic on one address of the memory costs some 20 ns, and all blocks of a row share it
+        if (threadIdx.x == 0) sh.n_list = 0;
+        __syncthreads();
+        look_gather(row, s.lo, s.hi, w.st.klo, sh.list, &sh.n_list);
+        to_row_list(sh, w);
         return;
     }
     for (int q = 0; q < kPer; ++q) sh.bins[q * kThreads + threadIdx.x] = 0;
@@ -1198,7 +1216,7 @@ __global__ __launch_bounds__(kThreads) void split_border_kernel(SampleArgs a, Ro
         if (n <= kBins) {
             for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.list[i] = w.list[i];
             __syncthreads();
-            draw_from_list(a, w.st.r, b, n, sh);
+            draw_from_list(a, row, w.st.r, b, n, w.st.klo, sh);
         } else {
             alone = true;
         }
@@ -1229,11 +1247,10 @@ __global__ __launch_bounds__(kThreads) void split_border_kernel(SampleArgs a, Ro
     if (threadIdx.x == 0) w.st.mode = kDone;
 }
 
-// Blocks over which a row is cut: enough to have two on each of the card's 256 compute units, segments of 4096 elements
-// (one step of a block) at least; 1: not cut.
+// Blocks over which a row is cut; 1: not cut.  SPLITRULE
 int splits(int64_t B, int64_t V) {
-    const int64_t c = std::min<int64_t>(std::min<int64_t>(512 / B, V / 4096), kMaxSplit);
-    return V > kSmall && c >= 2 ? (int)c : 1;
+    const int64_t c = std::min<int64_t>(512 / B, kMaxSplit);
+    return V >= 1 << 17 && c >= 8 ? (int)c : 1;
 }
 
 template <typename T>
@@ -1248,8 +1265,9 @@ void launch_split(const SampleArgs& a, int64_t B, int C, RowSpace* ws, hipStream
     hipLaunchKernelGGL(split_plan_kernel<T>, one, block, 0, st, a, ws, 64 * C);
     hipLaunchKernelGGL(split_look_kernel<T>, wide, block, 0, st, a, ws);
     hipLaunchKernelGGL(split_border_kernel<T>, one, block, 0, st, a, ws);
-    // rows that top_p may send over bins have one more look
-    if (sizeof(T) == 4 && (a.top_p || a.p < 1.0)) {
+    // rows that top_p may send over bins have one more look; none does whose top_k leads to a list
+    const bool listed = !a.top_k && a.k > 0 && a.k < a.V && by_maxima(a.k, 64 * C);
+    if (sizeof(T) == 4 && !listed && (a.top_p || a.p < 1.0)) {
         hipLaunchKernelGGL(split_look_kernel<T>, wide, block, 0, st, a, ws);
         hipLaunchKernelGGL(split_border_kernel<T>, one, block, 0, st, a, ws);
     }
