@@ -375,8 +375,7 @@ __device__ __forceinline__ void sort_list(uint32_t n, u64* list) {
 }
 
 // sort_list<true> for keys from klo to khi, by way of 4096 ranges of keys (in sh.count): a range's entries go to its place,
-// and the thread that owns the range puts its few in order.  Where many share a range, the bitonic way does it.  (1150
-// entries: MEASURE us, bitonic MEASURE us.)
+// and each to the one that its range's larger entries leave it.  Where many share a range, the bitonic way does it.
 __device__ __forceinline__ void sort_by_ranges(uint32_t n, uint32_t klo, uint32_t khi, Shared& sh) {
     if (n <= 256) return sort_list<true>(n, sh.list);
     const int bits = klo == khi ? 0 : 32 - __clz(khi - klo), shift = bits > 12 ? bits - 12 : 0;
@@ -400,28 +399,31 @@ __device__ __forceinline__ void sort_by_ranges(uint32_t n, uint32_t klo, uint32_
         most = std::max(most, c[q]);
         sum += c[q];
     }
-    if (__syncthreads_or(most > 16)) return sort_list<true>(n, sh.list);
-    const uint32_t first = (uint32_t)(block_incl(sum, sh, &all) - sum);
-    uint32_t at = first;
+    if (__syncthreads_or(most > 64)) return sort_list<true>(n, sh.list);
+    uint32_t at = (uint32_t)(block_incl(sum, sh, &all) - sum);
 #pragma unroll
     for (int q = 0; q < kPer; ++q) sh.count[kPer * threadIdx.x + q] = at, at += c[q];
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kPer; ++q)
-        if (q * kThreads + threadIdx.x < n) sh.list[sh.count[(khi - (uint32_t)(x[q] >> 32)) >> shift] + rank[q]] = x[q];
-    __syncthreads();
-    at = first;
+    uint32_t first[kPer], end[kPer];
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-        const uint32_t end = at + c[q];
-        for (uint32_t i = at + 1; i < end; ++i) {                    // insertion: the largest first
-            const u64 y = sh.list[i];
-            uint32_t j = i;
-            for (; j > at && sh.list[j - 1] < y; --j) sh.list[j] = sh.list[j - 1];
-            sh.list[j] = y;
-        }
-        at = end;
+        if (q * kThreads + threadIdx.x >= n) continue;
+        const uint32_t range = (khi - (uint32_t)(x[q] >> 32)) >> shift;
+        first[q] = sh.count[range];
+        end[q] = range + 1 < kBins ? sh.count[range + 1] : n;
+        sh.list[first[q] + rank[q]] = x[q];
     }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        if (q * kThreads + threadIdx.x >= n) continue;
+        rank[q] = first[q];
+        for (uint32_t i = first[q]; i < end[q]; ++i) rank[q] += sh.list[i] > x[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kPer; ++q)
+        if (q * kThreads + threadIdx.x < n) sh.list[rank[q]] = x[q];
     __syncthreads();
 }
 
@@ -470,12 +472,9 @@ __device__ __forceinline__ void draw_by_tiles(const SampleArgs& a, const T* row,
     __syncthreads();
     for (int q = wave; q < a.draws; q += kWaves) {
         const u64 want = draw_target(a, b * a.draws + q, total);
-        uint32_t lo = 0, hi = tiles - 1;
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (sh.tile[mid] > want) hi = mid;
-            else lo = mid + 1;
-        }
+        // the first tile whose running sum is above `want`: among each 64th, then among 64 (past the last tile all are above)
+        const uint32_t part = __ffsll((long long)__ballot(sh.tile[64 * lane + 63] > want)) - 1;
+        const uint32_t lo = 64 * part + __ffsll((long long)__ballot(sh.tile[64 * part + lane] > want)) - 1;
         u64 before = lo ? sh.tile[lo - 1] : 0;
         const uint32_t end = std::min(a.V, (lo + 1) * a.tile);
         bool found = false;
@@ -490,11 +489,17 @@ __device__ __forceinline__ void draw_by_tiles(const SampleArgs& a, const T* row,
             for (int g = 0; g < 4; ++g) {
                 if (found) continue;
                 u64 x[4], four = 0;
+                bool kept[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t i = i0 + 256 * g + 4 * lane + e;
-                    const bool kept = i < end && candidate(l[g][e]) && entry(key_of(l[g][e]), i) >= last && passes(r, l[g][e]);
-                    x[e] = kept ? weight(r, l[g][e], sh.tab) : 0;
+                    kept[e] = i < end && candidate(l[g][e]) && entry(key_of(l[g][e]), i) >= last && passes(r, l[g][e]);
+                }
+                if (!__any(kept[0] || kept[1] || kept[2] || kept[3])) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const u64 one = weight(r, l[g][e], sh.tab);
+                    x[e] = kept[e] ? one : 0;
                     four += x[e];
                 }
                 const u64 sums = before + wave_incl(four);
