@@ -8,6 +8,7 @@
 #include "hmx_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -16,6 +17,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxD = 32768;
+constexpr int64_t kFewRows = 2048;      // up to this many the backward pass is one launch
 constexpr int kBwdBlocks = 1024;      // rows of weight-gradient partials at most (4 blocks per CU)
 
 template <typename T>
@@ -78,19 +80,30 @@ __device__ __forceinline__ void load_weight(const float* p, float (&v)[VEC]) {
 
 // Sum over the LPR lanes that share a row, in every one of them.  LPR > 64: the block is one row; `red` holds one float
 // per wave and may be reused after the next call's first barrier.
-template <int LPR>
-__device__ __forceinline__ float row_sum(float v, float* red) {
+template <int LPR, typename S>
+__device__ __forceinline__ S row_sum(S v, S* red) {
 #pragma unroll
     for (int off = (LPR < 64 ? LPR : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off);
     if constexpr (LPR > 64) {
         __syncthreads();                                   // the previous row's sums have been read
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.f;
+        v = 0;
 #pragma unroll
         for (int i = 0; i < LPR / 64; ++i) v += red[i];
     }
     return v;
+}
+
+// fp64 to fp32 so that a later rounding to fewer bits comes out as if it were the only one: cut, and the last bit set where
+// anything was cut off.  fp32 stays as it is.
+__device__ __forceinline__ float round_to_odd(float v) { return v; }
+__device__ __forceinline__ float round_to_odd(double v) {
+    const float f = (float)v;
+    uint32_t u = __float_as_uint(f);
+    if ((double)f == v || f != f) return f;
+    if (fabs((double)f) > fabs(v)) --u;                                // rounded away from zero (to infinity: the largest number)
+    return __uint_as_float(u | 1);
 }
 
 // Least e with amax <= 448 * 2^e, -126 <= e <= 127 (0 for a block of zeros); 128 marks a block that is not finite.
@@ -105,16 +118,19 @@ __device__ __forceinline__ int mx8_exponent(float amax) {
 template <typename T, int VEC, int LPR, int NV, bool MX8>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void add_rmsnorm_fwd_kernel(
     const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr, const float* __restrict__ w, int64_t T_rows,
-    int d, float eps, T* __restrict__ s, T* __restrict__ y, float* __restrict__ rstd, uint8_t* __restrict__ codes,
+    int d, double eps, T* __restrict__ s, T* __restrict__ y, float* __restrict__ rstd, uint8_t* __restrict__ codes,
     uint8_t* __restrict__ scales, int dp) {
     constexpr int kRows = (LPR > 256 ? LPR : 256) / LPR;
-    __shared__ float red[LPR > 64 ? LPR / 64 : 1];
+    __shared__ typename std::conditional<MX8, double, float>::type red[LPR > 64 ? LPR / 64 : 1];
     const int l = threadIdx.x % LPR, slot = threadIdx.x / LPR;
     for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < T_rows; row0 += (int64_t)gridDim.x * kRows) {
         const int64_t row = row0 + slot;
         const bool ok = row < T_rows;
         float sv[NV][VEC];
-        float ss = 0.f;
+        // the 8-bit form rounds coarsely, and an error of y next to a rounding border becomes a whole step of it: statistics
+        // and y are fp64 there (a tenth of the time that the row's bytes take)
+        using Sum = typename std::conditional<MX8, double, float>::type;
+        Sum ss = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (l + LPR * i) * VEC;
@@ -133,9 +149,9 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void add_rmsnorm_fwd_kernel(
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) ss = fmaf(sv[i][e], sv[i][e], ss);
+            for (int e = 0; e < VEC; ++e) ss = fma((Sum)sv[i][e], (Sum)sv[i][e], ss);
         ss = row_sum<LPR>(ss, red);
-        const float inv = 1.f / sqrtf(ss / (float)d + eps);
+        const Sum inv = (Sum)1 / sqrt(ss / (Sum)d + (Sum)eps);
         if (ok && rstd && l == 0) rstd[row] = inv;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -148,7 +164,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void add_rmsnorm_fwd_kernel(
                 load_weight<VEC>(w + c, wv);
                 if (s) store_vec<T, VEC>(s + row * d + c, sv[i]);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) yv[e] = sv[i][e] * inv * wv[e];
+                for (int e = 0; e < VEC; ++e) yv[e] = round_to_odd((Sum)sv[i][e] * inv * (Sum)wv[e]);
                 if constexpr (!MX8) store_vec<T, VEC>(y + row * d + c, yv);
             }
             if constexpr (MX8) {
@@ -193,15 +209,36 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void add_rmsnorm_fwd_kernel(
     }
 }
 
-// g = dy * w;  dx = ds + rstd * (g - s rstd^2 mean(g s));  dw[c] = sum over rows dy s rstd (one row of partials a block).
+// g = dy * w;  dx = ds + rstd * (g - s rstd^2 mean(g s));  dw[c] = sum over rows dy s rstd.
+// Blocks below row_blocks take rows.  dw: long inputs, each of them leaves a row of partials in dw_part (summed by a second
+// launch); few rows (dw), one more block for each 16 columns reads them all once more, out of cache: a call of that size
+// costs what its launches and buffers cost the host.
 template <typename T, int VEC, int LPR, int NV>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void add_rmsnorm_bwd_kernel(
     const T* __restrict__ s, const float* __restrict__ w, const float* __restrict__ rstd, const T* __restrict__ dy,
-    const T* __restrict__ ds, int64_t T_rows, int d, T* __restrict__ dx, float* __restrict__ dw_part) {
+    const T* __restrict__ ds, int64_t T_rows, int d, T* __restrict__ dx, float* __restrict__ dw_part, float* __restrict__ dw_all,
+    int row_blocks) {
     constexpr int kThreads = LPR > 256 ? LPR : 256, kRows = kThreads / LPR;
     __shared__ float red[LPR > 64 ? LPR / 64 : 1];
-    __shared__ float dws[kRows > 1 ? kThreads * VEC : 1];
+    __shared__ float dws[kThreads * (kRows > 1 ? VEC : 1)];
     const int l = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+    if ((int)blockIdx.x >= row_blocks) {
+        const int c = ((int)blockIdx.x - row_blocks) * 16 + (int)(threadIdx.x & 15);
+        float a = 0.f;
+        if (c < d) {
+#pragma unroll 8
+            for (int64_t row = threadIdx.x >> 4; row < T_rows; row += kThreads / 16)
+                a = fmaf(Elem<T>::load(dy + row * d + c), Elem<T>::load(s + row * d + c) * rstd[row], a);
+        }
+        dws[threadIdx.x] = a;
+        __syncthreads();
+        if (threadIdx.x < 16 && c < d) {
+            a = 0.f;
+            for (int q = 0; q < kThreads / 16; ++q) a += dws[q * 16 + threadIdx.x];
+            dw_all[c] = a;
+        }
+        return;
+    }
     float dw[NV][VEC], wv[NV][VEC];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -210,7 +247,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void add_rmsnorm_bwd_kernel(
         for (int e = 0; e < VEC; ++e) dw[i][e] = wv[i][e] = 0.f;
         if (c < d) load_weight<VEC>(w + c, wv[i]);
     }
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < T_rows; row0 += (int64_t)gridDim.x * kRows) {
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < T_rows; row0 += (int64_t)row_blocks * kRows) {
         const int64_t row = row0 + slot;
         const bool ok = row < T_rows;
         float sv[NV][VEC], gv[NV][VEC];
@@ -277,6 +314,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void add_rmsnorm_bwd_kernel(
     }
 }
 
+// Blocks of the backward pass, each with a row of weight-gradient partials (none: no rows).
+int64_t bwd_blocks(int64_t T, int64_t d) {
+    return std::min<int64_t>(std::min<int64_t>(T, hmx_ceil_div(T * std::min<int64_t>(d, 1024), 1024)), kBwdBlocks);
+}
+
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 struct FwdArgs {
@@ -285,7 +327,7 @@ struct FwdArgs {
     const float* w;
     int64_t T;
     int d;
-    float eps;
+    double eps;
     void *s, *y;
     float* rstd;
     uint8_t *codes, *scales;
@@ -349,14 +391,15 @@ struct BwdArgs {
     int64_t T;
     int d;
     void* dx;
-    float* part;
+    float *part, *dw;
 };
 
 template <typename T, int VEC, int LPR, int NV>
 void launch_bwd(const BwdArgs& a, hipStream_t st) {
     constexpr int kThreads = LPR > 256 ? LPR : 256;
-    hipLaunchKernelGGL((add_rmsnorm_bwd_kernel<T, VEC, LPR, NV>), dim3((int)hmx_add_rmsnorm_bwd_blocks(a.T, a.d)), dim3(kThreads), 0,
-                       st, (const T*)a.s, a.w, a.rstd, (const T*)a.dy, (const T*)a.ds, a.T, a.d, (T*)a.dx, a.part);
+    const int rows = (int)bwd_blocks(a.T, a.d), more = a.dw ? (int)hmx_ceil_div(a.d, 16) : 0;
+    hipLaunchKernelGGL((add_rmsnorm_bwd_kernel<T, VEC, LPR, NV>), dim3(rows + more), dim3(kThreads), 0, st, (const T*)a.s, a.w, a.rstd,
+                       (const T*)a.dy, (const T*)a.ds, a.T, a.d, (T*)a.dx, a.part, a.dw, rows);
 }
 
 template <typename T>
@@ -386,9 +429,9 @@ bool bad_rows(int64_t T, int64_t d) { return T < 0 || d <= 0 || d > kMaxD; }
 
 // ================================================================================ C ABI
 extern "C" int hmx_add_rmsnorm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* scale, int64_t T,
-                                   int64_t d, float eps, int bf16, void* s, void* y, float* rstd, void* stream) {
+                                   int64_t d, double eps, int bf16, void* s, void* y, float* rstd, void* stream) {
     HMX_ENTER();
-    if (bad_rows(T, d) || !(eps >= 0.f)) return HMX_EINVAL;
+    if (bad_rows(T, d) || !(eps >= 0.0)) return HMX_EINVAL;
     if (T == 0) return HMX_OK;
     if (!x || !scale || !y || (residual && !s) || ldx < 0 || ldr < 0) return HMX_EINVAL;
     const FwdArgs a = {x, residual, ldx, residual ? ldr : 0, scale, T, (int)d, eps, s, y, rstd, nullptr, nullptr, 0};
@@ -396,9 +439,9 @@ extern "C" int hmx_add_rmsnorm_fwd(const void* x, int64_t ldx, const void* resid
 }
 
 extern "C" int hmx_add_rmsnorm_mx8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* scale, int64_t T,
-                                   int64_t d, float eps, int bf16, void* s, void* codes, void* scales, void* stream) {
+                                   int64_t d, double eps, int bf16, void* s, void* codes, void* scales, void* stream) {
     HMX_ENTER();
-    if (bad_rows(T, d) || !(eps >= 0.f)) return HMX_EINVAL;
+    if (bad_rows(T, d) || !(eps >= 0.0)) return HMX_EINVAL;
     if (T == 0) return HMX_OK;
     if (!x || !scale || !codes || !scales || (residual && !s) || ldx < 0 || ldr < 0) return HMX_EINVAL;
     const FwdArgs a = {x, residual, ldx, residual ? ldr : 0, scale, T, (int)d, eps, s, nullptr, nullptr, (uint8_t*)codes,
@@ -406,17 +449,28 @@ extern "C" int hmx_add_rmsnorm_mx8(const void* x, int64_t ldx, const void* resid
     return bf16 ? dispatch_fwd<__bf16, true>(a, (hipStream_t)stream) : dispatch_fwd<float, true>(a, (hipStream_t)stream);
 }
 
-extern "C" int64_t hmx_add_rmsnorm_bwd_blocks(int64_t T, int64_t d) {
-    if (T <= 0 || d <= 0) return 1;
-    return std::min<int64_t>(std::min<int64_t>(T, hmx_ceil_div(T * std::min<int64_t>(d, 1024), 1024)), kBwdBlocks);
+extern "C" size_t hmx_add_rmsnorm_bwd_workspace_bytes(int64_t T, int64_t d) {
+    if (T <= kFewRows || d <= 0) return 0;
+    const int64_t blocks = bwd_blocks(T, d);
+    return hmx_align_up((size_t)blocks * d * sizeof(float), 256) + hmx_colsum_workspace_bytes(blocks, d);
 }
 
 extern "C" int hmx_add_rmsnorm_bwd(const void* s, const float* scale, const float* rstd, const void* dy, const void* ds, int64_t T,
-                                   int64_t d, int bf16, void* dx, float* dscale_part, void* stream) {
+                                   int64_t d, int bf16, void* dx, float* dscale, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
     HMX_ENTER();
     if (bad_rows(T, d)) return HMX_EINVAL;
-    if (T == 0) return HMX_OK;
-    if (!s || !scale || !rstd || !dy || !dx) return HMX_EINVAL;
-    const BwdArgs a = {s, dy, ds, scale, rstd, T, (int)d, dx, dscale_part};
-    return bf16 ? dispatch_bwd<__bf16>(a, (hipStream_t)stream) : dispatch_bwd<float>(a, (hipStream_t)stream);
+    if (T > 0 && (!s || !scale || !rstd || !dy || !dx)) return HMX_EINVAL;
+    const size_t need = hmx_add_rmsnorm_bwd_workspace_bytes(T, d);
+    if (dscale && need > 0 && (!workspace || workspace_bytes < need)) return HMX_EWORKSPACE;
+    const hipStream_t st = (hipStream_t)stream;
+    if (T == 0) return dscale ? hmx_colsum_f32(nullptr, 0, d, d, dscale, nullptr, 0, stream) : HMX_OK;       // zeros
+    HmxCarver carve(workspace);
+    const int64_t blocks = bwd_blocks(T, d);
+    float* part = dscale && need > 0 ? carve.take<float>((size_t)(blocks * d)) : nullptr;
+    const BwdArgs a = {s, dy, ds, scale, rstd, T, (int)d, dx, part, part ? nullptr : dscale};
+    const int rc = bf16 ? dispatch_bwd<__bf16>(a, st) : dispatch_bwd<float>(a, st);
+    if (rc != HMX_OK || !part) return rc;
+    const size_t left = hmx_colsum_workspace_bytes(blocks, d);
+    return hmx_colsum_f32(part, blocks, d, d, dscale, left ? carve.take<char>(left) : nullptr, left, stream);
 }

@@ -109,20 +109,24 @@ def rmsnorm(x, scale, eps=1e-6):
     return _RMSNorm.apply(x, scale, eps)
 
 
+_NORM_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
 def _norm_operands(what, x, residual, scale, eps):
     """Checks the operands of the residual-add norms; -> device, (T, d) views of x and residual, 1 for bfloat16."""
     device = _one_device(what, x, residual, scale)
-    if x.dtype not in (torch.float32, torch.bfloat16):
+    shape, bf16 = x.shape, _NORM_DTYPES.get(x.dtype)
+    if bf16 is None:
         raise hmx.HmxError(f"{what}: x is float32 or bfloat16, got {x.dtype}")
-    if x.dim() == 0 or not 1 <= x.shape[-1] <= 32768:
-        raise hmx.HmxError(f"{what}: the last dimension of x holds 1 to 32768 values, got {tuple(x.shape)}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise hmx.HmxError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} does not match x {tuple(x.shape)} {x.dtype}")
-    if scale.shape != (x.shape[-1],) or scale.dtype != torch.float32:
-        raise hmx.HmxError(f"{what}: scale is float32 ({x.shape[-1]},), got {scale.dtype} {tuple(scale.shape)}")
+    if not shape or not 1 <= shape[-1] <= 32768:
+        raise hmx.HmxError(f"{what}: the last dimension of x holds 1 to 32768 values, got {tuple(shape)}")
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
+        raise hmx.HmxError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} does not match x {tuple(shape)} {x.dtype}")
+    if scale.shape != shape[-1:] or scale.dtype != torch.float32:
+        raise hmx.HmxError(f"{what}: scale is float32 ({shape[-1]},), got {scale.dtype} {tuple(scale.shape)}")
     if not eps >= 0.0:
         raise hmx.HmxError(f"{what}: eps is {eps}")
-    return device, _rows(x), None if residual is None else _rows(residual), int(x.dtype == torch.bfloat16)
+    return device, _rows(x), None if residual is None else _rows(residual), bf16
 
 
 class _AddRMSNorm(torch.autograd.Function):
@@ -145,26 +149,23 @@ class _AddRMSNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, ds=None):
-        s, scale, rstd = ctx.saved_tensors
         if dy is None:                            # nothing arrives at y: the sum passes its own gradient on
             return ds, (ds if ctx.has_residual else None), None, None
-        device, d = s.device, s.shape[-1]
-        s2, dy2 = _rows(s).contiguous(), dy.reshape(-1, d).contiguous()
-        ds2 = None if ds is None else ds.reshape(-1, d).contiguous()
-        T = s2.shape[0]
+        s, scale, rstd = ctx.saved_tensors
+        device, d, T = s.device, s.shape[-1], rstd.shape[0]
+        s, dy = s.contiguous(), dy.contiguous()
+        if ds is not None:
+            ds = ds.contiguous()
         dx = torch.empty(s.shape, dtype=s.dtype, device=device)
-        dscale = None
-        part = None
+        dscale = ws = None
+        nbytes = 0
         if ctx.needs_input_grad[2]:
-            if T:
-                part = torch.empty(_L().hmx_add_rmsnorm_bwd_blocks(T, d), d, dtype=torch.float32, device=device)
-            else:
-                dscale = torch.zeros(d, dtype=torch.float32, device=device)
-        _launch("hmx_add_rmsnorm_bwd", device, s2.data_ptr(), scale.data_ptr(), rstd.data_ptr(), dy2.data_ptr(), hmx.ptr(ds2), T,
-                d, ctx.bf16, dx.data_ptr(), hmx.ptr(part))
-        if part is not None:
-            with torch.cuda.device(device):
-                dscale = colsum(part)
+            dscale = torch.empty(d, dtype=torch.float32, device=device)
+            nbytes = _L().hmx_add_rmsnorm_bwd_workspace_bytes(T, d)
+            if nbytes:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _launch("hmx_add_rmsnorm_bwd", device, s.data_ptr(), scale.data_ptr(), rstd.data_ptr(), dy.data_ptr(), hmx.ptr(ds), T, d,
+                ctx.bf16, dx.data_ptr(), hmx.ptr(dscale), hmx.ptr(ws), nbytes)
         return dx, (dx if ctx.has_residual else None), dscale, None
 
 

@@ -152,10 +152,10 @@ PROTOTYPES = {
     "hmx_dropout_multiplier_f32": (c_int, [ctypes.c_uint64, ctypes.c_uint64, I64, F, P, P]),
     "hmx_attn_fwd": (c_int, [P, P, P, I64, I64, I64, I64, I64, P, P, P]),
     "hmx_attn_bwd": (c_int, [P, P, P, P, P, I64, I64, I64, I64, I64, P, P, P, P, P]),
-    "hmx_add_rmsnorm_fwd": (c_int, [P, I64, P, I64, P, I64, I64, F, c_int, P, P, P, P]),
-    "hmx_add_rmsnorm_bwd_blocks": (I64, [I64, I64]),
-    "hmx_add_rmsnorm_bwd": (c_int, [P, P, P, P, P, I64, I64, c_int, P, P, P]),
-    "hmx_add_rmsnorm_mx8": (c_int, [P, I64, P, I64, P, I64, I64, F, c_int, P, P, P, P]),
+    "hmx_add_rmsnorm_fwd": (c_int, [P, I64, P, I64, P, I64, I64, ctypes.c_double, c_int, P, P, P, P]),
+    "hmx_add_rmsnorm_bwd_workspace_bytes": (c_size_t, [I64, I64]),
+    "hmx_add_rmsnorm_bwd": (c_int, [P, P, P, P, P, I64, I64, c_int, P, P, P, c_size_t, P]),
+    "hmx_add_rmsnorm_mx8": (c_int, [P, I64, P, I64, P, I64, I64, ctypes.c_double, c_int, P, P, P, P]),
     "hmx_mx4_quantize": (c_int, [P, I64, I64, I64, c_int, P, P, P]),
     "hmx_mx_dequantize": (c_int, [P, P, I64, I64, c_int, c_int, P, P]),
     "hmx_linear_mx4": (c_int, [P, I64, P, c_int, I64, P, P, I64, I64, c_int, P, P]),

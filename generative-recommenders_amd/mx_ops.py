@@ -22,7 +22,6 @@ def padded(d):
     return -(-d // BLOCK) * BLOCK
 
 
-@torch.no_grad()
 def add_rmsnorm_mx8(x, residual, scale, eps=1e-6):
     """enc_ops.add_rmsnorm with y in mx8 -> (codes float8_e4m3fn (..., dp), scales uint8 (..., dp / 32), s); residual
     None: s is x.  The codes come from the float32 y; no gradient."""
@@ -67,19 +66,16 @@ def _dequantize(what, bits, codes, scales, d, dtype):
     return out
 
 
-@torch.no_grad()
 def dequantize_mx8(codes, scales, d=None, dtype=torch.bfloat16):
     """The values that mx8 codes stand for, (..., d); d None: all dp of them.  bfloat16 holds each exactly."""
     return _dequantize("dequantize_mx8", 8, codes, scales, d, dtype)
 
 
-@torch.no_grad()
 def dequantize_mx4(codes, scales, d=None, dtype=torch.bfloat16):
     """The values that mx4 codes stand for, (..., d); d None: all dp of them.  bfloat16 holds each exactly."""
     return _dequantize("dequantize_mx4", 4, codes, scales, d, dtype)
 
 
-@torch.no_grad()
 def quantize_mx4(table):
     """table (..., d) float32 or bfloat16 -> (codes uint8 (..., dp / 2), scales uint8 (..., dp / 32)).  Run it again
     after the table's weights changed."""
@@ -99,7 +95,6 @@ def quantize_mx4(table):
 _X_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
 
 
-@torch.no_grad()
 def linear_mx4(x, codes, scales, x_scales=None, out_dtype=torch.float32):
     """out (..., N) = x (..., K) times the transposed mx4 table (codes (N, dp / 2), scales (N, dp / 32)), dp = padded(K).
 

@@ -30,28 +30,32 @@ def _i64c(t):
     return t.contiguous()
 
 
-def _one_device(what, *tensors):
+def _one_device(what, first, *others):
     """The GPU that every tensor given (None: left out) lies on; raises when one lies elsewhere."""
-    _need_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise hmx.HmxError(f"{what}: the tensors lie on different devices ({', '.join(sorted(map(str, devices)))})")
-    return devices.pop()
+    device = first.device
+    if device.type != "cuda" or any(t is not None and t.device != device for t in others):
+        _need_cuda(first, *others)
+        raise hmx.HmxError(f"{what}: the tensors lie on different devices: "
+                           f"{', '.join(str(t.device) for t in (first, *others) if t is not None)}")
+    return device
 
 
 def _launch(name, device, *args):
     """Calls an entry point on `device` and its current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        code = getattr(hmx.lib(), name)(*args, hmx.current_stream())
+    index = device.index
+    fn = getattr(hmx.lib(), name)
+    if index == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            code = getattr(hmx.lib(), name)(*args, hmx.current_stream())
-    hmx.check(code, name)
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code != 0:
+        hmx.check(code, name)
 
 
 def _rows(t):
     """(..., d) as a (rows, d) view whose columns are contiguous (a copy only where the strides allow no such view)."""
-    t2 = t.reshape(-1, t.shape[-1])
+    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     return t2 if t2.stride(1) == 1 or t2.shape[1] == 1 else t2.contiguous()
 
 
@@ -577,7 +581,6 @@ def _row_setting(what, name, value, dtype, n_rows, device):
     return value.contiguous(), 0
 
 
-@torch.no_grad()
 def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Draws items from rows of scores -> (ids int64, probs float32), both of u's shape.
 

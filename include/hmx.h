@@ -653,14 +653,13 @@ int hmx_attn_bwd(const float* q, const float* kv, const float* drop, const float
  * (T, d) with row strides ldx / ldr in elements (0: one row for all), s, y contiguous.  residual NULL: the norm of x
  * (s may then be NULL).  rstd (T) or NULL receives the factor for the backward pass.  1 <= d <= 32768, eps >= 0. */
 int hmx_add_rmsnorm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* scale, int64_t T,
-                        int64_t d, float eps, int bf16, void* s, void* y, float* rstd, void* stream);
+                        int64_t d, double eps, int bf16, void* s, void* y, float* rstd, void* stream);
 
 /* Its gradient: dx (T, d), the gradient of x and of residual alike, from dy and ds (NULL: no gradient arrives at s), all
- * contiguous; dscale_part (hmx_add_rmsnorm_bwd_blocks(T, d), d) or NULL receives partial rows whose column sums
- * (hmx_colsum_f32) are the gradient of scale. */
-int64_t hmx_add_rmsnorm_bwd_blocks(int64_t T, int64_t d);
+ * contiguous, and dscale (d) or NULL (then no workspace is needed). */
+size_t hmx_add_rmsnorm_bwd_workspace_bytes(int64_t T, int64_t d);
 int hmx_add_rmsnorm_bwd(const void* s, const float* scale, const float* rstd, const void* dy, const void* ds, int64_t T,
-                        int64_t d, int bf16, void* dx, float* dscale_part, void* stream);
+                        int64_t d, int bf16, void* dx, float* dscale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Block-scaled formats: 32 consecutive values of a row share one scale byte b that stands for 2^(b - 127); "mx8" holds a
  * value as e4m3 (a byte), "mx4" as e2m1 (half a byte: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign; the value with the even
@@ -669,9 +668,9 @@ int hmx_add_rmsnorm_bwd(const void* s, const float* scale, const float* rstd, co
  * no value is cut off; values are rounded to nearest even.  A block that holds a NaN or an infinity gets scale byte 255
  * and zero codes, and stands for NaN.  Codes and scales are contiguous, codes 16-byte aligned.
  *
- * hmx_add_rmsnorm_mx8: hmx_add_rmsnorm_fwd with y in mx8 (from the unrounded fp32 y): codes (T, dp), scales (T, dp / 32). */
+ * hmx_add_rmsnorm_mx8: hmx_add_rmsnorm_fwd with y in mx8, rounded once from the fp64 value: codes (T, dp), scales (T, dp / 32). */
 int hmx_add_rmsnorm_mx8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* scale, int64_t T,
-                        int64_t d, float eps, int bf16, void* s, void* codes, void* scales, void* stream);
+                        int64_t d, double eps, int bf16, void* s, void* codes, void* scales, void* stream);
 
 /* A (n, d) table (fp32, or bfloat16 where bf16 = 1; row stride ld in elements) in mx4: codes (n, dp / 2), scales
  * (n, dp / 32), and the values that mx4 (bits = 4) or mx8 (bits = 8) codes stand for, (n, d) fp32 or bfloat16: exact in

@@ -21,12 +21,15 @@ def test_norm_entries():
     assert L.hmx_add_rmsnorm_fwd(*a, None, P, None, None) == EINVAL          # a residual without a place for the sum
     assert L.hmx_add_rmsnorm_fwd(*a, P, None, None, None) == EINVAL
     assert L.hmx_add_rmsnorm_mx8(*a, P, None, P, None) == EINVAL
-    assert L.hmx_add_rmsnorm_bwd(P, P, None, P, None, 4, 64, 0, P, None, None) == EINVAL
-    assert L.hmx_add_rmsnorm_bwd(P, P, P, P, None, 4, 40000, 0, P, None, None) == EINVAL
+    bwd = dict(s=P, w=P, rstd=P, dy=P, ds=None, T=4, d=64, bf16=0, dx=P, dw=None, ws=None, ws_bytes=0, stream=None)
+    for bad in (dict(s=None), dict(w=None), dict(rstd=None), dict(dy=None), dict(dx=None), dict(T=-1), dict(d=40000)):
+        assert L.hmx_add_rmsnorm_bwd(*{**bwd, **bad}.values()) == EINVAL
+    nbytes = L.hmx_add_rmsnorm_bwd_workspace_bytes(10 ** 5, 64)
+    assert nbytes > 0 and L.hmx_add_rmsnorm_bwd_workspace_bytes(4, 64) == 0
+    for bad in (dict(dw=P), dict(dw=P, ws=P, ws_bytes=nbytes - 1), dict(dw=P, ws=None, ws_bytes=nbytes)):
+        assert L.hmx_add_rmsnorm_bwd(*{**bwd, "T": 10 ** 5, **bad}.values()) == -2
     assert L.hmx_add_rmsnorm_fwd(None, 64, None, 0, None, 0, 64, 0.0, 0, None, None, None, None) == 0
-    assert L.hmx_add_rmsnorm_bwd(None, None, None, None, None, 0, 64, 0, None, None, None) == 0
-    for T in (0, 1, 5, 10 ** 6):
-        assert 1 <= L.hmx_add_rmsnorm_bwd_blocks(T, 64) <= max(T, 1)
+    assert L.hmx_add_rmsnorm_bwd(*{**bwd, "T": 0, "s": None}.values()) == 0
 
 
 def test_mx4_entries():
