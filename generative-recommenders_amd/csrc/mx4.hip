@@ -171,19 +171,40 @@ struct XTerms {
     bf16x8 p[PL];
 };
 
-// x[m, k .. k + 7] as exact bf16 terms; columns past K and rows past M read as zero.  VEC: the rows are 16-byte aligned.
-template <int XK, bool VEC>
+// v = h + m + l exactly: each term is the next 8 bits of the significand (cut, not rounded: no carry, and the largest finite
+// value stays finite).  An infinity or a NaN stays in the first term alone.
+__device__ __forceinline__ XTerms<3> cut3(const float (&v)[8]) {
+    uint32_t u[3][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        uint32_t b = __float_as_uint(v[e]);
+        const bool fin = (b & 0x7f800000u) != 0x7f800000u;
+        if (!fin && (b & 0x7fffffu)) b |= 0x400000u;                 // a NaN whose payload would be cut away
+        u[0][e] = b & 0xffff0000u;
+        const float r1 = fin ? v[e] - __uint_as_float(u[0][e]) : 0.f;
+        u[1][e] = __float_as_uint(r1) & 0xffff0000u;
+        u[2][e] = __float_as_uint(r1 - __uint_as_float(u[1][e]));
+    }
+    XTerms<3> t;
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (u[q][2 * e] >> 16) | (u[q][2 * e + 1] & 0xffff0000u);
+        t.p[q] = __builtin_bit_cast(bf16x8, w);
+    }
+    return t;
+}
+
+// x[m, k .. k + 7] as exact bf16 terms; columns past K and rows past M read as zero.
+template <int XK>
 __device__ __forceinline__ XTerms<planes<XK>()> load_x8(const LinearArgs& a, int m, int k) {
     XTerms<planes<XK>()> t;
     const bool row = m < a.M;
     if constexpr (XK == kXBf16) {
         const __bf16* p = (const __bf16*)a.x + m * a.ldx + k;
-        if (VEC && row && k + 8 <= a.K) {
-            t.p[0] = *reinterpret_cast<const bf16x8*>(p);
-        } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) t.p[0][e] = row && k + e < a.K ? p[e] : (__bf16)0.f;
-        }
+        for (int e = 0; e < 8; ++e) t.p[0][e] = row && k + e < a.K ? p[e] : (__bf16)0.f;
     } else if constexpr (XK == kXMx8) {
         f32x8 v;
         if (row && k < a.K) {                                           // K = 32 * nblk
@@ -200,34 +221,9 @@ __device__ __forceinline__ XTerms<planes<XK>()> load_x8(const LinearArgs& a, int
     } else {
         const float* p = (const float*)a.x + m * a.ldx + k;
         float v[8];
-        if (VEC && row && k + 8 <= a.K) {
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = row && k + e < a.K ? p[e] : 0.f;
-        }
-        // v = h + m + l exactly: each term is the next 8 bits of the significand (cut, not rounded: no carry, and the
-        // largest finite value stays finite).  An infinity or a NaN stays in the first term alone.
-        uint32_t u[3][8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            uint32_t b = __float_as_uint(v[e]);
-            const bool fin = (b & 0x7f800000u) != 0x7f800000u;
-            if (!fin && (b & 0x7fffffu)) b |= 0x400000u;                // a NaN whose payload would be cut away
-            u[0][e] = b & 0xffff0000u;
-            const float r1 = fin ? v[e] - __uint_as_float(u[0][e]) : 0.f;
-            u[1][e] = __float_as_uint(r1) & 0xffff0000u;
-            u[2][e] = __float_as_uint(r1 - __uint_as_float(u[1][e]));
-        }
-#pragma unroll
-        for (int q = 0; q < 3; ++q) {
-            u32x4 w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = (u[q][2 * e] >> 16) | (u[q][2 * e + 1] & 0xffff0000u);
-            t.p[q] = __builtin_bit_cast(bf16x8, w);
-        }
+        for (int e = 0; e < 8; ++e) v[e] = row && k + e < a.K ? p[e] : 0.f;
+        t = cut3(v);
     }
     return t;
 }
@@ -270,7 +266,7 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
         if constexpr (REP) {
             const int jr = c >> 2, ir = c & 3;
             const bool mine = R == 1 || (R == 2 ? (j >> 1) == (jr & 1) : j == jr);
-            const XTerms<PL> t = load_x8<XK, false>(a, mine ? (PL == 3 ? 0 : ir) : a.M, 32 * b + 8 * i);
+            const XTerms<PL> t = load_x8<XK>(a, mine ? (PL == 3 ? 0 : ir) : a.M, 32 * b + 8 * i);
             if constexpr (PL == 3) {
                 xr[i][0] = zero_if(ir != 0, t.p[0]);
                 xr[i][0] = ir == 1 ? t.p[1] : xr[i][0];
@@ -279,7 +275,7 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
                 xr[i][0] = t.p[0];
             }
         } else {
-            const XTerms<PL> t = load_x8<XK, false>(a, mbase + c, 32 * b + 8 * i);
+            const XTerms<PL> t = load_x8<XK>(a, mbase + c, 32 * b + 8 * i);
 #pragma unroll
             for (int q = 0; q < PL; ++q) xr[i][q] = t.p[q];
         }
@@ -381,8 +377,76 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
     }
 }
 
+// The 32 values of a row of x that one lane multiplies with its block of W, as they lie in memory.
+template <int XK>
+struct XBlock;
+template <>
+struct XBlock<kXF32> {
+    f32x4 v[8];
+    __device__ __forceinline__ XTerms<3> octet(int i) const {
+        const f32x4 lo = v[2 * i], hi = v[2 * i + 1];
+        const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        return cut3(f);
+    }
+};
+template <>
+struct XBlock<kXBf16> {
+    bf16x8 v[4];
+    __device__ __forceinline__ XTerms<1> octet(int i) const { return XTerms<1>{{v[i]}}; }
+};
+template <>
+struct XBlock<kXMx8> {
+    u32x4 v[2];
+    uint32_t scale;
+    __device__ __forceinline__ XTerms<1> octet(int i) const {
+        const float s = scale_value(scale);
+        const uint32_t lo = v[i / 2][2 * (i & 1)], hi = v[i / 2][2 * (i & 1) + 1];
+        u32x4 w;
+        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
+        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true));
+        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false));
+        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
+        return XTerms<1>{{__builtin_bit_cast(bf16x8, w)}};
+    }
+};
+
+// x[m, 32 b .. 32 b + 31], zero past K; m and b lie in the tensor.  VEC: rows are 16-byte aligned.
+template <int XK, bool VEC>
+__device__ __forceinline__ XBlock<XK> load_x_block(const LinearArgs& a, int m, int b) {
+    XBlock<XK> t;
+    if constexpr (XK == kXMx8) {
+        const u32x4* p = reinterpret_cast<const u32x4*>((const uint8_t*)a.x + (int64_t)m * a.K + 32 * b);
+        t.v[0] = p[0], t.v[1] = p[1];
+        t.scale = a.xs[(int64_t)m * a.nblk + b];
+    } else if constexpr (XK == kXBf16) {
+        const __bf16* p = (const __bf16*)a.x + m * a.ldx + 32 * b;
+        if (VEC && 32 * b + 32 <= a.K) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t.v[i] = reinterpret_cast<const bf16x8*>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t.v[i][e] = 32 * b + 8 * i + e < a.K ? p[8 * i + e] : (__bf16)0.f;
+        }
+    } else {
+        const float* p = (const float*)a.x + m * a.ldx + 32 * b;
+        if (VEC && 32 * b + 32 <= a.K) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t.v[i] = reinterpret_cast<const f32x4*>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t.v[i][e] = 32 * b + 4 * i + e < a.K ? p[4 * i + e] : 0.f;
+        }
+    }
+    return t;
+}
+
 // Longer rows: eight waves a block, KW of them share 16 RT rows of the table and split its K (pairs of 128 columns in turn,
-// so that a wave reads whole 128-byte lines); their sums meet in LDS and are added in wave order.
+// so that a wave reads whole 128-byte lines); their sums meet in LDS and are added in wave order.  The loads of the next
+// 128 columns are in flight while these are multiplied.
 template <int XK, int MT, int RT, bool VEC, typename OUT>
 __global__ __launch_bounds__(512) void linear_long_kernel(LinearArgs a, int KW) {
     constexpr int PL = planes<XK>(), NE = RT * MT * 4;
@@ -400,39 +464,62 @@ __global__ __launch_bounds__(512) void linear_long_kernel(LinearArgs a, int KW) 
     int64_t row_at[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) row_at[r] = (n0 + 16 * r + c < a.N ? n0 + 16 * r + c : a.N - 1) * a.nblk;
-    if (n0 < a.N) {
-        for (int c0 = 2 * kw; c0 < chunks; c0 += 2 * KW) {
-            u32x4 w[2][RT];
-            uint32_t sc[2][RT];
+    int mrow[MT];                                                    // rows past M are not stored: any row will do
 #pragma unroll
-            for (int p = 0; p < 2; ++p)
+    for (int m = 0; m < MT; ++m) mrow[m] = mbase + 16 * m + c < a.M ? mbase + 16 * m + c : a.M - 1;
+    struct Chunk {
+        u32x4 w[RT];
+        uint32_t sc[RT];
+        XBlock<XK> x[MT];
+        bool ok;
+    };
+    auto fetch = [&](int n, Chunk& t) {                              // the n-th chunk of this wave
+        const int b = 4 * (2 * (kw + KW * (n >> 1)) + (n & 1)) + j;
+        t.ok = b < a.nblk;
+        const int bb = t.ok ? b : 0;
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    const int b = 4 * (c0 + p) + j;
-                    const int64_t at = row_at[r] + (b < a.nblk ? b : 0);
-                    w[p][r] = a.codes[at];
-                    sc[p][r] = a.scales[at];
-                }
+        for (int r = 0; r < RT; ++r) {
+            t.w[r] = a.codes[row_at[r] + bb];
+            t.sc[r] = a.scales[row_at[r] + bb];
+        }
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const int b = 4 * (c0 + p) + j;
-                const bool ok = b < a.nblk;
+        for (int m = 0; m < MT; ++m) t.x[m] = load_x_block<XK, VEC>(a, mrow[m], bb);
+    };
+    auto multiply = [&](const Chunk& t) {
+        float s[RT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    XTerms<PL> xt[MT];
+        for (int r = 0; r < RT; ++r) s[r] = t.ok ? scale_value(t.sc[r]) : 1.f;
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) xt[m] = load_x8<XK, VEC>(a, ok ? mbase + 16 * m + c : a.M, ok ? 32 * b + 8 * i : 0);
+        for (int i = 0; i < 4; ++i) {
+            XTerms<PL> xt[MT];
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        const bf16x8 wv = decode_bf16(ok ? w[p][r][i] : 0u, ok ? scale_value(sc[p][r]) : 1.f);
+            for (int m = 0; m < MT; ++m) {
+                xt[m] = t.x[m].octet(i);
 #pragma unroll
-                        for (int m = 0; m < MT; ++m)
-#pragma unroll
-                            for (int q = 0; q < PL; ++q)
-                                acc[r][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xt[m].p[q], wv, acc[r][m], 0, 0, 0);
-                    }
-                }
+                for (int q = 0; q < PL; ++q) xt[m].p[q] = zero_if(!t.ok, xt[m].p[q]);
             }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const bf16x8 wv = decode_bf16(t.ok ? t.w[r][i] : 0u, s[r]);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int q = 0; q < PL; ++q)
+                        acc[r][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xt[m].p[q], wv, acc[r][m], 0, 0, 0);
+            }
+        }
+    };
+    // chunks of this wave (an odd one out counts: its lanes past the row multiply zeros)
+    const int pairs = (chunks + 1) / 2, mine = 2 * ((pairs - kw + KW - 1) / KW);
+    if (n0 < a.N && mine > 0) {
+        Chunk even, odd;
+        fetch(0, even);
+#pragma unroll 1
+        for (int n = 0; n < mine; n += 2) {
+            fetch(n + 1, odd);
+            multiply(even);
+            if (n + 2 < mine) fetch(n + 2, even);
+            multiply(odd);
         }
     }
 #pragma unroll
@@ -475,7 +562,8 @@ void launch_linear(const LinearArgs& a, bool vec, hipStream_t st) {
     hipLaunchKernelGGL((linear_long_kernel<XK, MT, RT, VEC, OUT>),                                                       \
                        dim3((unsigned)hmx_ceil_div(a.N, 16 * RT * (8 / kw)), (unsigned)hmx_ceil_div(a.M, 16 * MT)), dim3(512), 0, \
                        st, a, kw)
-    if (a.M <= 16) { if (vec) LONG(1, 2, true); else LONG(1, 2, false); }
+    // two tiles of 16 rows of x a wave share what decoding W costs; the three terms of fp32 leave no registers for that
+    if (a.M <= 16 || XK == kXF32) { if (vec) LONG(1, 2, true); else LONG(1, 2, false); }
     else { if (vec) LONG(2, 2, true); else LONG(2, 2, false); }
 #undef LONG
 }
