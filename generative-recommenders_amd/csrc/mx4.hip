@@ -247,6 +247,17 @@ __device__ __forceinline__ bf16x8 zero_if(bool z, bf16x8 v) {
 template <typename OUT>
 __device__ __forceinline__ void store_out(OUT* p, float v) { *p = (OUT)v; }
 
+// v[t] of lane group j becomes v[j] of lane group t (groups of 16 lanes).
+__device__ __forceinline__ void transpose_groups(float (&v)[4]) {
+    typedef uint32_t pair __attribute__((ext_vector_type(2)));
+    uint32_t u[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) u[t] = __float_as_uint(v[t]);
+    const pair a = __builtin_amdgcn_permlane32_swap(u[0], u[2], false, false), b = __builtin_amdgcn_permlane32_swap(u[1], u[3], false, false);
+    const pair c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    v[0] = __uint_as_float(c[0]), v[1] = __uint_as_float(c[1]), v[2] = __uint_as_float(d[0]), v[3] = __uint_as_float(d[1]);
+}
+
 // K <= 128 (scores of a table of embeddings): x stays in registers, waves walk the table 64 rows at a time.
 // With one or two blocks a row (R = 4 or 2), the lane groups of one load hold R groups of 16 rows, so that a load still is
 // 1 KB of consecutive codes; the MFMA would add the groups up, so x is zero in the lane groups of the other row groups:
@@ -362,13 +373,16 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
                 }
             }
         } else {
+            // lane group j holds rows 4 j + i of each 16 table rows: exchanged, so that a store is 64 consecutive scores
+            const int64_t n = tile * 64 + lane;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int64_t n = tile * 64 + t * 16 + c;
+            for (int i = 0; i < 4; ++i) {
+                float v[4] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+                transpose_groups(v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int m = mbase + 4 * j + i;
-                    if (n < a.N && m < a.M) store_out(out + m * a.N + n, acc[t][i]);
+                for (int g = 0; g < 4; ++g) {
+                    const int m = mbase + 4 * g + i;
+                    if (n < a.N && m < a.M) store_out(out + m * a.N + n, v[g]);
                 }
             }
         }
@@ -377,85 +391,39 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
     }
 }
 
-// The 32 values of a row of x that one lane multiplies with its block of W, as they lie in memory.
+// Longer rows go in two launches.  The first lays x out as the second one's lanes take it: per tile of 16 operand rows and
+// 128 columns, step i and lane, the eight bf16 values of one MFMA operand.  An fp32 row is three operand rows (its terms; five
+// rows of x to a tile), any other one.  Read as it lies, x cost more than W: rows of a power of two of bytes lie in one
+// memory channel and one set of the cache, and every block decodes all of x (32 x 8192 x 8192 mx8: 22 us, this way 15 and 3).
 template <int XK>
-struct XBlock;
-template <>
-struct XBlock<kXF32> {
-    f32x4 v[8];
-    __device__ __forceinline__ XTerms<3> octet(int i) const {
-        const f32x4 lo = v[2 * i], hi = v[2 * i + 1];
-        const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        return cut3(f);
-    }
-};
-template <>
-struct XBlock<kXBf16> {
-    bf16x8 v[4];
-    __device__ __forceinline__ XTerms<1> octet(int i) const { return XTerms<1>{{v[i]}}; }
-};
-template <>
-struct XBlock<kXMx8> {
-    u32x4 v[2];
-    uint32_t scale;
-    __device__ __forceinline__ XTerms<1> octet(int i) const {
-        const float s = scale_value(scale);
-        const uint32_t lo = v[i / 2][2 * (i & 1)], hi = v[i / 2][2 * (i & 1) + 1];
-        u32x4 w;
-        w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
-        w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true));
-        w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false));
-        w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
-        return XTerms<1>{{__builtin_bit_cast(bf16x8, w)}};
-    }
-};
-
-// x[m, 32 b .. 32 b + 31], zero past K; m and b lie in the tensor.  VEC: rows are 16-byte aligned.
-template <int XK, bool VEC>
-__device__ __forceinline__ XBlock<XK> load_x_block(const LinearArgs& a, int m, int b) {
-    XBlock<XK> t;
-    if constexpr (XK == kXMx8) {
-        const u32x4* p = reinterpret_cast<const u32x4*>((const uint8_t*)a.x + (int64_t)m * a.K + 32 * b);
-        t.v[0] = p[0], t.v[1] = p[1];
-        t.scale = a.xs[(int64_t)m * a.nblk + b];
-    } else if constexpr (XK == kXBf16) {
-        const __bf16* p = (const __bf16*)a.x + m * a.ldx + 32 * b;
-        if (VEC && 32 * b + 32 <= a.K) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t.v[i] = reinterpret_cast<const bf16x8*>(p)[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) t.v[i][e] = 32 * b + 8 * i + e < a.K ? p[8 * i + e] : (__bf16)0.f;
-        }
-    } else {
-        const float* p = (const float*)a.x + m * a.ldx + 32 * b;
-        if (VEC && 32 * b + 32 <= a.K) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t.v[i] = reinterpret_cast<const f32x4*>(p)[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) t.v[i][e] = 32 * b + 4 * i + e < a.K ? p[4 * i + e] : 0.f;
-        }
-    }
-    return t;
+__global__ __launch_bounds__(256) void linear_pack_kernel(LinearArgs a, int chunks, int64_t total, u32x4* __restrict__ packed) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= total) return;
+    const int lane = (int)(t & 63), i = (int)(t >> 6) & 3, r = lane & 15;
+    const int64_t unit = t >> 8;
+    const int chunk = (int)(unit % chunks), tile = (int)(unit / chunks);
+    const int m = XK == kXF32 ? tile * 5 + r / 3 : tile * 16 + r;
+    if ((XK == kXF32 && r == 15) || m >= a.M) return;                // lanes that the second launch leaves out
+    const XTerms<planes<XK>()> x = load_x8<XK>(a, m, 256 * (chunk >> 1) + 64 * (lane >> 4) + 32 * (chunk & 1) + 8 * i);
+    bf16x8 v = x.p[0];
+    if constexpr (XK == kXF32) v = r % 3 == 1 ? x.p[1] : r % 3 == 2 ? x.p[2] : v;
+    packed[t] = __builtin_bit_cast(u32x4, v);
 }
 
-// Longer rows: eight waves a block, KW of them share 16 RT rows of the table and split its K (pairs of 128 columns in turn,
-// so that a wave reads whole 128-byte lines); their sums meet in LDS and are added in wave order.  The loads of the next
-// 128 columns are in flight while these are multiplied.
-template <int XK, int MT, int RT, bool VEC, typename OUT>
-__global__ __launch_bounds__(512) void linear_long_kernel(LinearArgs a, int KW) {
-    constexpr int PL = planes<XK>(), NE = RT * MT * 4;
-    __shared__ float red[8][NE][64];
+// What lanes past the end of a row load in place of codes and scales.
+__device__ const u32x4 kZeros = {};
+
+// The second: W waves a block, KW of them share 16 RT rows of the table and split its K (256 columns in turn, two chunks of
+// 128 of which a lane has two neighbouring blocks: a wave reads whole 128-byte lines); their sums meet in LDS and are added in
+// wave order.  The next chunk is in flight while one is multiplied.  TERMS: operand rows of a row of x.
+template <int TERMS, int W, int MT, int RT, typename OUT>
+__global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const u32x4* __restrict__ packed, int KW) {
+    constexpr int NE = RT * MT * 4, ROWS = TERMS == 3 ? 5 : 16;      // rows of x to a tile
+    __shared__ float red[W][NE][64];
     const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4, wave = threadIdx.x >> 6;
     const int kw = wave % KW, group = wave / KW;
-    const int64_t n0 = ((int64_t)blockIdx.x * (8 / KW) + group) * (16 * RT);
-    const int mbase = blockIdx.y * (16 * MT);
-    const int chunks = (a.nblk + 3) / 4;
+    const int64_t n0 = ((int64_t)blockIdx.x * (W / KW) + group) * (16 * RT);
+    const int chunks = 2 * ((a.nblk + 7) / 8);
     f32x4 acc[RT][MT];
 #pragma unroll
     for (int r = 0; r < RT; ++r)
@@ -464,62 +432,80 @@ __global__ __launch_bounds__(512) void linear_long_kernel(LinearArgs a, int KW) 
     int64_t row_at[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) row_at[r] = (n0 + 16 * r + c < a.N ? n0 + 16 * r + c : a.N - 1) * a.nblk;
-    int mrow[MT];                                                    // rows past M are not stored: any row will do
+    bool used[MT];                                                   // operand rows that there are; the others are zero
 #pragma unroll
-    for (int m = 0; m < MT; ++m) mrow[m] = mbase + 16 * m + c < a.M ? mbase + 16 * m + c : a.M - 1;
+    for (int m = 0; m < MT; ++m) {
+        const int left = a.M - (int)(blockIdx.y * MT + m) * ROWS;
+        used[m] = c < TERMS * (left < ROWS ? left : ROWS);
+    }
+    // blocks begin at different columns: rows of a power of two of bytes lie in the same memory channel column by column, and
+    // blocks in step would all wait for it
+    const int pairs = chunks / 2, mine = 2 * ((pairs - kw + KW - 1) / KW), turn = (int)(blockIdx.x * 37u % (unsigned)pairs);
     struct Chunk {
-        u32x4 w[RT];
-        uint32_t sc[RT];
-        XBlock<XK> x[MT];
-        bool ok;
+        u32x4 w[RT], x[MT][4];
+    };
+    uint32_t sc[RT];                                                 // both chunks' scales, the second's in the upper byte
+    const int64_t all = a.N * a.nblk;
+    auto pair_of = [&](int n) {
+        const int pair = kw + KW * (n >> 1) + turn;
+        return pair < pairs ? pair : pair - pairs;
     };
     auto fetch = [&](int n, Chunk& t) {                              // the n-th chunk of this wave
-        const int b = 4 * (2 * (kw + KW * (n >> 1)) + (n & 1)) + j;
-        t.ok = b < a.nblk;
-        const int bb = t.ok ? b : 0;
+        const int chunk = 2 * pair_of(n) + (n & 1), b = 4 * (chunk & ~1) + 2 * j + (chunk & 1);
+        const bool past = b >= a.nblk;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) t.w[r] = *(past ? &kZeros : a.codes + row_at[r] + b);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const u32x4* p = packed + (((int64_t)(blockIdx.y * MT + m) * chunks + chunk) * 4) * 64 + lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                t.x[m][i] = u32x4{0, 0, 0, 0};
+                if (used[m] && !past) t.x[m][i] = p[64 * i];
+            }
+        }
+    };
+    auto fetch_scales = [&](int n, uint32_t (&sd)[RT]) {             // of the pair that the n-th chunk begins
+        const int b = 8 * pair_of(n) + 2 * j;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            t.w[r] = a.codes[row_at[r] + bb];
-            t.sc[r] = a.scales[row_at[r] + bb];
+            const int64_t at = row_at[r] + b;
+            uint16_t two = 0;
+            if (at + 2 <= all) __builtin_memcpy(&two, a.scales + at, 2);
+            else if (b < a.nblk) two = a.scales[at];
+            sd[r] = b + 1 < a.nblk ? two : b < a.nblk ? two & 255u : 0u;
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) t.x[m] = load_x_block<XK, VEC>(a, mrow[m], bb);
     };
-    auto multiply = [&](const Chunk& t) {
+    auto multiply = [&](const Chunk& t, int half) {
         float s[RT];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) s[r] = t.ok ? scale_value(t.sc[r]) : 1.f;
+        for (int r = 0; r < RT; ++r) s[r] = scale_value((sc[r] >> (8 * half)) & 255u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            XTerms<PL> xt[MT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                xt[m] = t.x[m].octet(i);
-#pragma unroll
-                for (int q = 0; q < PL; ++q) xt[m].p[q] = zero_if(!t.ok, xt[m].p[q]);
-            }
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                const bf16x8 wv = decode_bf16(t.ok ? t.w[r][i] : 0u, s[r]);
+                const bf16x8 wv = decode_bf16(t.w[r][i], s[r]);
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int q = 0; q < PL; ++q)
-                        acc[r][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xt[m].p[q], wv, acc[r][m], 0, 0, 0);
+                    acc[r][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.x[m][i]), wv, acc[r][m], 0, 0, 0);
             }
-        }
     };
-    // chunks of this wave (an odd one out counts: its lanes past the row multiply zeros)
-    const int pairs = (chunks + 1) / 2, mine = 2 * ((pairs - kw + KW - 1) / KW);
     if (n0 < a.N && mine > 0) {
         Chunk even, odd;
+        uint32_t next[RT];
         fetch(0, even);
+        fetch_scales(0, sc);
 #pragma unroll 1
         for (int n = 0; n < mine; n += 2) {
             fetch(n + 1, odd);
-            multiply(even);
-            if (n + 2 < mine) fetch(n + 2, even);
-            multiply(odd);
+            multiply(even, 0);
+            if (n + 2 < mine) {
+                fetch(n + 2, even);
+                fetch_scales(n + 2, next);
+            }
+            multiply(odd, 1);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) sc[r] = next[r];
         }
     }
 #pragma unroll
@@ -530,19 +516,31 @@ __global__ __launch_bounds__(512) void linear_long_kernel(LinearArgs a, int KW) 
             for (int i = 0; i < 4; ++i) red[wave][(r * MT + m) * 4 + i][lane] = acc[r][m][i];
     __syncthreads();
     OUT* out = (OUT*)a.out;
-    for (int e = kw; e < NE; e += KW) {
+    for (int e = kw * 64 + lane; e < RT * MT * ROWS * 16; e += KW * 64) {
+        const int col = e & 15, q = (e >> 4) % ROWS, rm = (e >> 4) / ROWS;
         float v = 0.f;
-        for (int q = 0; q < KW; ++q) v += red[group * KW + q][e][lane];
-        const int r = e / (MT * 4), m = mbase + 16 * ((e / 4) % MT) + 4 * j + (e & 3);
-        const int64_t n = n0 + 16 * r + c;
+#pragma unroll
+        for (int p = 0; p < TERMS; ++p) {
+            const int row = TERMS * q + p;
+            float sum = 0.f;
+            for (int k = 0; k < KW; ++k) sum += red[group * KW + k][rm * 4 + (row & 3)][(row >> 2) * 16 + col];
+            v += sum;
+        }
+        const int m = ((int)blockIdx.y * MT + rm % MT) * ROWS + q;
+        const int64_t n = n0 + 16 * (rm / MT) + col;
         if (n < a.N && m < a.M) store_out(out + m * a.N + n, v);
     }
 }
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+constexpr int kWavesLong = 8;
+
+// Tiles of 16 operand rows that M rows of x make for linear_long_kernel.
+int operand_tiles(int x_kind, int64_t M) { return (int)hmx_ceil_div(M, x_kind == kXF32 ? 5 : 16); }
+
 template <int XK, typename OUT>
-void launch_linear(const LinearArgs& a, bool vec, hipStream_t st) {
+void launch_linear(const LinearArgs& a, u32x4* packed, hipStream_t st) {
     if (a.nblk <= 4) {
         const bool rep = XK == kXF32 ? a.M == 1 : a.M <= 4;
         const int64_t want = hmx_ceil_div(hmx_ceil_div(a.N, 64), 4);
@@ -555,16 +553,20 @@ void launch_linear(const LinearArgs& a, bool vec, hipStream_t st) {
 #undef SHORT
         return;
     }
-    const int chunks = (a.nblk + 3) / 4;
-    int kw = 8;
+    const int chunks = 2 * (int)hmx_ceil_div(a.nblk, 8), tiles = operand_tiles(XK, a.M);
+    const int64_t total = (int64_t)tiles * chunks * 256;
+    hipLaunchKernelGGL(linear_pack_kernel<XK>, dim3((unsigned)hmx_ceil_div(total, 256)), dim3(256), 0, st, a, chunks, total, packed);
+    int kw = kWavesLong;
     while (kw > 1 && chunks < 4 * kw) kw /= 2;
-#define LONG(MT, RT, VEC)                                                                                              \
-    hipLaunchKernelGGL((linear_long_kernel<XK, MT, RT, VEC, OUT>),                                                       \
-                       dim3((unsigned)hmx_ceil_div(a.N, 16 * RT * (8 / kw)), (unsigned)hmx_ceil_div(a.M, 16 * MT)), dim3(512), 0, \
-                       st, a, kw)
-    // two tiles of 16 rows of x a wave share what decoding W costs; the three terms of fp32 leave no registers for that
-    if (a.M <= 16 || XK == kXF32) { if (vec) LONG(1, 2, true); else LONG(1, 2, false); }
-    else { if (vec) LONG(2, 2, true); else LONG(2, 2, false); }
+#define LONG(MT, RT)                                                                                                      \
+    hipLaunchKernelGGL((linear_long_kernel<planes<XK>(), kWavesLong, MT, RT, OUT>),                                       \
+                       dim3((unsigned)hmx_ceil_div(a.N, 16 * RT * (kWavesLong / kw)), (unsigned)hmx_ceil_div(tiles, MT)), \
+                       dim3(64 * kWavesLong), 0, st, a, packed, kw)
+    // two tiles of x a wave share what decoding W costs, two of W what loading x does; one of W where two would leave compute
+    // units without a block (32 x 4096 x 4096 mx8: 9.0 us against 10.4)
+    const bool wide = hmx_ceil_div(a.N, 32 * (kWavesLong / kw)) >= 256;
+    if (tiles == 1) { if (wide) LONG(1, 2); else LONG(1, 1); }
+    else { if (wide) LONG(2, 2); else LONG(2, 1); }
 #undef LONG
 }
 
@@ -621,8 +623,15 @@ extern "C" int hmx_mx_dequantize(const void* codes, const void* scales, int64_t 
     return HMX_OK;
 }
 
+extern "C" size_t hmx_linear_mx4_workspace_bytes(int x_kind, int64_t M, int64_t K) {
+    if (M <= 0 || K <= 128) return 0;
+    const int64_t tiles = hmx_ceil_div(operand_tiles(x_kind, M), 2) * 2;      // read in twos
+    return (size_t)(tiles * hmx_ceil_div(K, 256) * 2) * 4096;
+}
+
 extern "C" int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, int x_kind, int64_t M, const void* codes,
-                              const void* scales, int64_t N, int64_t K, int out_bf16, void* out, void* stream) {
+                              const void* scales, int64_t N, int64_t K, int out_bf16, void* out, void* workspace,
+                              size_t workspace_bytes, void* stream) {
     HMX_ENTER();
     if (M < 0 || N < 0 || K < 1 || K > (1 << 26) || ldx < 0 || x_kind < 0 || x_kind > 2) return HMX_EINVAL;
     if (M == 0 || N == 0) return HMX_OK;
@@ -631,11 +640,12 @@ extern "C" int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, 
     if (x_kind == kXMx8 && (K % 32 || !aligned(x, 16))) return HMX_EINVAL;
     const LinearArgs a = {x, ldx, (const uint8_t*)x_scales, (int)M, (const u32x4*)codes, (const uint8_t*)scales, N, (int)K,
                           (int)hmx_ceil_div(K, 32), out};
-    const bool vec = aligned(x, 16) && (ldx * (x_kind == kXF32 ? 4 : 2)) % 16 == 0;
+    const size_t need = hmx_linear_mx4_workspace_bytes(x_kind, M, K);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return HMX_EWORKSPACE;
     const hipStream_t st = (hipStream_t)stream;
-#define LINEAR(XK)                                          \
-    if (out_bf16) launch_linear<XK, __bf16>(a, vec, st);    \
-    else launch_linear<XK, float>(a, vec, st)
+#define LINEAR(XK)                                                          \
+    if (out_bf16) launch_linear<XK, __bf16>(a, (u32x4*)workspace, st);      \
+    else launch_linear<XK, float>(a, (u32x4*)workspace, st)
     if (x_kind == kXF32) { LINEAR(kXF32); }
     else if (x_kind == kXBf16) { LINEAR(kXBf16); }
     else { LINEAR(kXMx8); }

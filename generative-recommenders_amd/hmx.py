@@ -158,7 +158,8 @@ PROTOTYPES = {
     "hmx_add_rmsnorm_mx8": (c_int, [P, I64, P, I64, P, I64, I64, ctypes.c_double, c_int, P, P, P, P]),
     "hmx_mx4_quantize": (c_int, [P, I64, I64, I64, c_int, P, P, P]),
     "hmx_mx_dequantize": (c_int, [P, P, I64, I64, c_int, c_int, P, P]),
-    "hmx_linear_mx4": (c_int, [P, I64, P, c_int, I64, P, P, I64, I64, c_int, P, P]),
+    "hmx_linear_mx4_workspace_bytes": (c_size_t, [c_int, I64, I64]),
+    "hmx_linear_mx4": (c_int, [P, I64, P, c_int, I64, P, P, I64, I64, c_int, P, P, c_size_t, P]),
     "hmx_sample_logits": (c_int, [P, I64, I64, I64, c_int, P, c_int, I64, P, P, P, P, ctypes.c_double, I64, ctypes.c_double,
                                   ctypes.c_double, P, P, P, c_size_t, P]),
     "hmx_sample_logits_workspace_bytes": (c_size_t, [I64, I64]),

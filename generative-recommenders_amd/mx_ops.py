@@ -123,6 +123,8 @@ def linear_mx4(x, codes, scales, x_scales=None, out_dtype=torch.float32):
     if padded(k) != blocks * BLOCK:
         raise hmx.HmxError(f"linear_mx4: rows of {k} values do not match a table of {blocks} blocks of {BLOCK}")
     out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=device)
+    nbytes = 0 if k <= 128 else hmx.lib().hmx_linear_mx4_workspace_bytes(kind, m, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _launch("hmx_linear_mx4", device, x2.data_ptr(), x2.stride(0), hmx.ptr(x_scales), kind, m, codes.data_ptr(),
-            scales.data_ptr(), n, k, int(out_dtype == torch.bfloat16), out.data_ptr())
+            scales.data_ptr(), n, k, int(out_dtype == torch.bfloat16), out.data_ptr(), hmx.ptr(ws), nbytes)
     return out

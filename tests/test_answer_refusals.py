@@ -41,10 +41,14 @@ def test_mx4_entries():
     assert L.hmx_mx4_quantize(None, 64, 0, 64, 0, None, None, None) == 0
     assert L.hmx_mx_dequantize(P, P, 4, 64, 6, 0, P, None) == EINVAL
     assert L.hmx_mx_dequantize(P, None, 4, 64, 4, 0, P, None) == EINVAL
-    good = dict(x=P, ldx=64, xs=None, kind=0, M=4, codes=P, scales=P, N=8, K=64, bf16=0, out=P, stream=None)
+    good = dict(x=P, ldx=64, xs=None, kind=0, M=4, codes=P, scales=P, N=8, K=64, bf16=0, out=P, ws=None, ws_bytes=0, stream=None)
     for bad in (dict(x=None), dict(kind=3), dict(kind=2), dict(xs=P), dict(kind=2, xs=P, K=60), dict(M=-1), dict(N=-1), dict(K=0),
                 dict(codes=P + 8), dict(scales=None), dict(out=None), dict(N=1 << 40), dict(M=1 << 30), dict(ldx=-1)):
         assert L.hmx_linear_mx4(*{**good, **bad}.values()) == EINVAL, bad
+    nbytes = L.hmx_linear_mx4_workspace_bytes(0, 4, 1000)
+    assert nbytes > 0 and L.hmx_linear_mx4_workspace_bytes(0, 4, 128) == 0
+    for bad in (dict(ws=P, ws_bytes=nbytes - 1), dict(ws=None, ws_bytes=nbytes), dict(ws=P + 8, ws_bytes=nbytes)):
+        assert L.hmx_linear_mx4(*{**good, "K": 1000, "ldx": 1000, **bad}.values()) == -2
     assert L.hmx_linear_mx4(*{**good, "M": 0}.values()) == 0
 
 
