@@ -545,7 +545,11 @@ void launch_linear(const LinearArgs& a, u32x4* packed, hipStream_t st) {
         const bool rep = XK == kXF32 ? a.M == 1 : a.M <= 4;
         const int64_t want = hmx_ceil_div(hmx_ceil_div(a.N, 64), 4);
         const unsigned my = (unsigned)hmx_ceil_div(a.M, 16);
-        const dim3 grid((unsigned)std::min<int64_t>(want, 2048), rep ? 1 : my);
+        // few enough blocks that one round holds them (a wave's start, x from memory into registers, costs 3 us), and where the
+        // output is wide fewer still: its write streams disturb each other.  Measured with 512 / 1024 / 2048 blocks: 1 x
+        // 4,000,001 x 64 fp32 38 / 33 / 37 us, 16 x 1,000,003 x 60 bf16 26 / 30 / 37 us.
+        const int64_t most = rep ? 1024 : std::max<int64_t>(1, 512 / my);
+        const dim3 grid((unsigned)std::min<int64_t>(want, most), rep ? 1 : my);
 #define SHORT(R, REP) hipLaunchKernelGGL((linear_short_kernel<XK, R, REP, OUT>), grid, dim3(256), 0, st, a)
         if (a.nblk == 1) { if (rep) SHORT(4, true); else SHORT(4, false); }
         else if (a.nblk == 2) { if (rep) SHORT(2, true); else SHORT(2, false); }
