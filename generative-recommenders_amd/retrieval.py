@@ -332,3 +332,65 @@ class ShardedRetriever:
             return ops.kth_largest(vals, k)
         union = vals.permute(1, 0, 2).reshape(qc, -1)
         return union.topk(k, dim=1).values[:, k - 1].contiguous()
+
+
+class SampledRetriever:
+    """Draws items for users from their scores over an item table that is kept in 4 bits, on one GPU.
+
+    sample(states, u) -> (ids int64, probs float32), both of u's shape: scores are states times the table's transpose (mx4
+    values, fp32 sums), draws follow ops.sample_logits (temperature, top_k, top_p, min_p; numbers or one per state).  Against
+    search() of ShardedRetriever, which returns the best k, this explores: probs is what each item was drawn with.  The
+    table takes 17 / 32 of a byte per value (a quarter of its bf16 copy); scores of a chunk of states are held in memory,
+    `score_bytes` of them at most."""
+
+    def __init__(self, table, id_offset=0, score_bytes=1 << 30):
+        self.id_offset = int(id_offset)
+        self.score_bytes = int(score_bytes)
+        self.refresh(table)
+
+    def refresh(self, table):
+        """Call after the table's weights changed (quantises it again)."""
+        from . import mx_ops
+        self.dim = table.shape[1]
+        self.codes, self.scales = mx_ops.quantize_mx4(table.detach())
+
+    def scores(self, states, norm_scale=None, residual=None, eps=1e-6):
+        """(n, d) states -> (n, items) fp32 scores.  norm_scale (d,): the states are first added to `residual` (where given)
+        and RMS-normalised, into 8 bits (mx_ops.add_rmsnorm_mx8)."""
+        from . import hmx, mx_ops
+        if states.dim() != 2 or states.shape[1] != self.dim:
+            raise hmx.HmxError(f"SampledRetriever: states are (n, {self.dim}), got {tuple(states.shape)}")
+        if norm_scale is None:
+            if residual is not None:
+                raise hmx.HmxError("SampledRetriever: a residual needs norm_scale")
+            return mx_ops.linear_mx4(states.detach(), self.codes, self.scales)
+        x, x_scales, _ = mx_ops.add_rmsnorm_mx8(states.detach(), None if residual is None else residual.detach(),
+                                                norm_scale.detach(), eps)
+        return mx_ops.linear_mx4(x, self.codes, self.scales, x_scales=x_scales)
+
+    def sample(self, states, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, exclude=None, norm_scale=None, residual=None,
+               eps=1e-6):
+        """u (n,) or (n, draws) in [0, 1): the random numbers.  exclude (n, any) int64: item ids never drawn for a state
+        (entries outside the table are ignored).  A state without a drawable item gets id -1."""
+        from . import hmx, ops
+        n, items = states.shape[0], self.codes.shape[0]
+        if u.shape[:1] != (n,) or u.dim() > 2:
+            raise hmx.HmxError(f"SampledRetriever: u is ({n},) or ({n}, draws), got {tuple(u.shape)}")
+        settings = (temperature, top_k, top_p, min_p)
+        step = max(1, self.score_bytes // (4 * max(1, items)))
+        ids = torch.empty(u.shape, dtype=torch.int64, device=u.device)
+        probs = torch.empty(u.shape, dtype=torch.float32, device=u.device)
+        for lo in range(0, n, step):
+            part = slice(lo, min(lo + step, n))
+            sc = self.scores(states[part], norm_scale, None if residual is None else residual[part], eps)
+            if exclude is not None:
+                row = exclude[part] - self.id_offset
+                inside = (row >= 0) & (row < items)
+                # an entry outside the table writes to its row's last column what that column holds already
+                keep = sc.gather(1, torch.full_like(row, items - 1))
+                sc.scatter_reduce_(1, torch.where(inside, row, items - 1), torch.where(inside, float("-inf"), keep), "amin")
+            t, k, p, mp = (s[part] if isinstance(s, torch.Tensor) else s for s in settings)
+            ids[part], probs[part] = ops.sample_logits(sc, u[part], t, k, p, mp)
+        if self.id_offset:
+            ids = torch.where(ids >= 0, ids + self.id_offset, ids)
+        return ids, probs
