@@ -254,7 +254,7 @@ struct Shared {
     State st;
     u64 wsum[kWaves], wsums[4][kWaves];
     float wmax[kWaves];
-    u64 above, in_bin;
+    u64 above;
     uint32_t bin, n_list, at;
 };
 
@@ -314,17 +314,17 @@ __device__ __forceinline__ float block_sum(float v, Shared& sh) {
 }
 
 // The place among four values a thread (in thread order) at which their running sum reaches `target` (> 0): sh.bin (kBins
-// where they do not), sh.above before it, sh.in_bin its value.  `extra` comes before the second half of the values.
+// where they do not), sh.above before it.  `extra` comes before the second half of the values.
 __device__ __forceinline__ void find_place(const u64 (&v)[kPer], u64 target, u64 extra, Shared& sh) {
     u64 all, sum = 0;
 #pragma unroll
     for (int q = 0; q < kPer; ++q) sum += v[q];
     u64 upto = block_incl(sum, sh, &all) - sum + (threadIdx.x >= kThreads / 2 ? extra : 0);
-    if (threadIdx.x == 0) sh.bin = kBins, sh.above = all + extra, sh.in_bin = 0;
+    if (threadIdx.x == 0) sh.bin = kBins, sh.above = all + extra;
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-        if (upto < target && target <= upto + v[q]) sh.bin = kPer * threadIdx.x + q, sh.above = upto, sh.in_bin = v[q];
+        if (upto < target && target <= upto + v[q]) sh.bin = kPer * threadIdx.x + q, sh.above = upto;
         upto += v[q];
     }
     __syncthreads();
@@ -436,7 +436,7 @@ __device__ __forceinline__ uint32_t place_of_mass(const Row& r, uint32_t n, u64 
         v[q] = i < n ? weight(r, entry_value(sh.list[i]), sh.tab) : 0;
     }
     find_place(v, target, 0, sh);
-    return std::min(sh.bin, n - 1);
+    return n ? std::min(sh.bin, n - 1) : 0;
 }
 
 __device__ __forceinline__ u64 draw_target(const SampleArgs& a, int64_t at, u64 total) {
@@ -788,7 +788,7 @@ __device__ __forceinline__ void narrow(const SampleArgs& a, const T* row, const 
         for (int q = 0; q < kPer; ++q) v[q] = sh.bins[kPer * threadIdx.x + q];
         find_place(v, *need, 0, sh);
         *need -= sh.above;
-        *khi -= sh.bin << shift;
+        *khi -= std::min<uint32_t>(sh.bin, kBins - 1) << shift;
         const uint32_t width = (1u << shift) - 1;
         klo = *khi - klo > width ? *khi - width : klo;
         __syncthreads();
@@ -1303,11 +1303,22 @@ __global__ __launch_bounds__(kThreads) void split_border_kernel(SampleArgs a, Ro
     if (threadIdx.x == 0) w.st.mode = kDone;
 }
 
-// Blocks over which a row is cut; 1: not cut.  SPLITRULE
+// Blocks over which a row is cut; 1: not cut.  One block's time grows with the row, a cut row costs four to six launches, and
+// from some 64 rows on the rows fill the card by themselves.  Measured, us, one block a row / cut (spread 3, T = 1):
+//                         top_k 50 fp32   top_p 0.9 fp32   no border fp32   top_p 0.9 bf16
+//    1 x    32,768         15 /  20         28 /  32         17 / 17          24 / 27
+//    1 x    65,536         19 /  21         41 /  32         26 / 17          33 / 27
+//    1 x   131,072         25 /  24         70 /  33         46 / 17          52 / 28
+//    1 x 1,000,000        114 /  26        443 /  43        307 / 22         298 / 34
+//   64 x   131,072         27 /  28         72 /  66         47 / 32          53 / 39
+//  128 x   131,072         36 /  43         79 /  92         54 / 48          53 / 49
 int splits(int64_t B, int64_t V) {
-    const int64_t c = std::min<int64_t>(512 / B, kMaxSplit);
-    return V >= 1 << 17 && c >= 8 ? (int)c : 1;
+    const int64_t c = std::min<int64_t>(std::min<int64_t>(512 / B, V / 4096), kMaxSplit);
+    return V >= 1 << 16 && c >= 8 ? (int)c : 1;
 }
+
+// Whether every row's top_k is sure to lead to a list (no looks by bins), for `groups` groups of maxima.
+bool listed(const SampleArgs& a, int groups) { return !a.top_k && a.k > 0 && a.k < a.V && by_maxima(a.k, groups); }
 
 template <typename T>
 void launch_split(const SampleArgs& a, int64_t B, int C, RowSpace* ws, hipStream_t st) {
@@ -1322,8 +1333,7 @@ void launch_split(const SampleArgs& a, int64_t B, int C, RowSpace* ws, hipStream
     hipLaunchKernelGGL(split_look_kernel<T>, wide, block, 0, st, a, ws);
     hipLaunchKernelGGL(split_border_kernel<T>, one, block, 0, st, a, ws);
     // rows that top_p may send over bins have one more look; none does whose top_k leads to a list
-    const bool listed = !a.top_k && a.k > 0 && a.k < a.V && by_maxima(a.k, 64 * C);
-    if (sizeof(T) == 4 && !listed && (a.top_p || a.p < 1.0)) {
+    if (sizeof(T) == 4 && !listed(a, 64 * C) && (a.top_p || a.p < 1.0)) {
         hipLaunchKernelGGL(split_look_kernel<T>, wide, block, 0, st, a, ws);
         hipLaunchKernelGGL(split_border_kernel<T>, one, block, 0, st, a, ws);
     }
@@ -1349,7 +1359,7 @@ extern "C" int hmx_sample_logits(const void* logits, int64_t ld, int64_t B, int6
     if (workspace_bytes < hmx_sample_logits_workspace_bytes(B, V) || (C > 1 && !workspace)) return HMX_EWORKSPACE;
     SampleArgs a = {logits, ld, (uint32_t)V, u, u_f64 != 0, (int)draws, temperature, top_p, min_p, top_k, temperature_all,
                     top_p_all, min_p_all, top_k_all, ids, probs, (uint32_t)(hmx_ceil_div(V, (int64_t)kBins * kTile) * kTile)};
-    if (C > 1) {
+    if (C > 1 && (bf16 || V >= 1 << 17 || !listed(a, kThreads))) {
         if (bf16) launch_split<__bf16>(a, B, C, (RowSpace*)workspace, (hipStream_t)stream);
         else launch_split<float>(a, B, C, (RowSpace*)workspace, (hipStream_t)stream);
     } else if (bf16) {

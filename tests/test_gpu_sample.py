@@ -204,6 +204,41 @@ def test_item_table_rows(setting, dtype):
     check(logits, u, **setting)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [3000, 65537, 140001])
+def test_temperatures_at_the_ends(V, dtype):
+    """Almost the highest score alone, almost equal weights, and a spread of scores near the type's range.  (Shares that no
+    whole number of equal weights makes: 21 of 30 equal ones are 0.7 itself.)"""
+    logits, u = rows(3, V, 6, dtype, seed=V + 1)
+    for t in (1e-30, 1e-3, 1e30):
+        for setting in (dict(), dict(k=30), dict(p=0.7303), dict(k=2501, p=0.7303), dict(mp=0.5)):
+            check(logits, u, t=t, **setting)
+    check(logits * 1e37, u, t=3e37, p=0.9)
+    check(logits * 1e-37, u, t=1e-37, k=40, p=0.9)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,V", [(70, 66000), (2, 65535), (2, 65536), (5, 131071), (64, 70001)])
+def test_rows_about_where_they_are_cut(B, V, dtype):
+    logits, u = rows(B, V, 2, dtype, seed=B)
+    for setting in (dict(), dict(k=50), dict(p=0.9), dict(k=3000, p=0.9), dict(mp=0.02)):
+        ids, probs = ops.sample_logits(logits, u, setting.get("t", 1.0), setting.get("k", 0), setting.get("p", 1.0), setting.get("mp", 0.0))
+        some = slice(0, B, max(1, B // 3))
+        want = check(logits[some], u[some], **setting)
+        assert torch.equal(ids[some], want[0]) and torch.equal(probs[some], want[1])
+
+
+def test_scores_in_order():
+    """Sorted rows: the kept set lies in a few tiles, and groups of neighbours are not alike."""
+    for V in (5000, 100001, 300001):
+        logits, u = rows(2, V, 20, seed=V)
+        for desc in (False, True):
+            ordered = torch.sort(logits, dim=1, descending=desc).values
+            for setting in (dict(k=100), dict(k=1500, p=0.9), dict(p=0.9), dict(k=2500)):
+                check(ordered, u, **setting)
+                check(ordered.bfloat16(), u, **setting)
+
+
 def test_many_rows_and_draws():
     logits, u = rows(600, 333, 3, seed=4)
     check(logits[:40], u[:40], k=30, p=0.9)
