@@ -10,7 +10,7 @@
 //
 // What bounds it: at four cycles a wave an instruction per element costs 0.9 us for 33.5 M elements on the whole card, so the
 // few instructions that every element meets come first, the 25 of a weight where they can be spared:
-//   bfloat16: one look counts the 16-bit values (4096 counters for 2^-6 <= |l| < 2^10, a list for the rest), which gives
+//   bfloat16: one look counts the 16-bit values (8192 counters for 2^-22 <= |l| < 2^10, a list for the rest), which gives
 //     every border exactly: a value and how many of its elements are kept.
 //   fp32, top_k: the k-th largest of the maxima of groups of elements is a value that at least k elements reach; what
 //     reaches it is gathered into a list, and the list does the rest (top_p and min_p on top of top_k included).
@@ -37,7 +37,8 @@ constexpr int kMaxSplit = 64;              // blocks a row is cut over at most (
 constexpr uint32_t kLowestKey = 0x00800000u;        // the key after that of -infinity
 constexpr float kMaxFloat = 3.402823466e38f;
 constexpr float kRange = 32.f;             // bins reach down to exp(-32) of the largest weight
-constexpr uint32_t kFirstMag = (127 - 6) << 7;      // bfloat16 magnitudes with a counter: 2^-6 up to 2^10
+constexpr uint32_t kFirstMag = (127 - 22) << 7;     // bfloat16 magnitudes with a counter: 2^-22 up to 2^10
+constexpr int kValues = 2 * 4096, kPerValue = kValues / kThreads;
 
 typedef unsigned long long u64;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -88,8 +89,8 @@ struct Raw<__bf16> {
 };
 
 // f(four values, index of the first) for the elements of [lo, hi), hi >= 4, by `threads` threads (all of them take part in
-// every step; values outside are NaN), DEPTH steps' loads in flight.  The body stays one step of code, the last step its
-// masking apart: most users run it a few times only, and then fetching instructions is what it costs.
+// every step; values outside are NaN), DEPTH steps' loads in flight.  The loop is unrolled over these: a load's register must
+// not be moved while it is awaited.
 template <int DEPTH, typename T, typename F>
 __device__ __forceinline__ void each_element(const T* row, uint32_t lo, uint32_t hi, int thread, int threads, F f) {
     const uint32_t stride = threads * 4, steps = (hi - lo + stride - 1) / stride, last = hi - 4;
@@ -98,19 +99,22 @@ __device__ __forceinline__ void each_element(const T* row, uint32_t lo, uint32_t
 #pragma unroll
     for (int q = 0; q < DEPTH; ++q) ahead[q].load(row + std::min(i + q * stride, last));
 #pragma unroll 1
-    for (uint32_t n = 0; n < steps; ++n, i += stride) {
-        const Raw<T> v = ahead[0];
+    for (uint32_t n = 0; n < steps; n += DEPTH) {
 #pragma unroll
-        for (int q = 0; q + 1 < DEPTH; ++q) ahead[q] = ahead[q + 1];
-        ahead[DEPTH - 1].load(row + std::min(i + DEPTH * stride, last));
-        float l[4] = {v.get(0), v.get(1), v.get(2), v.get(3)};
-        uint32_t first = i;
-        if (n + 1 == steps) {                       // past the end: the row's last four, without what came before
-            first = std::min(i, last);
+        for (int q = 0; q < DEPTH; ++q) {
+            if (n + q >= steps) break;
+            float l[4] = {ahead[q].get(0), ahead[q].get(1), ahead[q].get(2), ahead[q].get(3)};
+            uint32_t first = i;
+            if (n + q + 1 == steps) {               // past the end: the row's last four, without what came before
+                first = std::min(i, last);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) l[e] = first + e >= i ? l[e] : __builtin_nanf("");
+                for (int e = 0; e < 4; ++e) l[e] = first + e >= i ? l[e] : __builtin_nanf("");
+            } else {
+                ahead[q].load(row + std::min(i + DEPTH * stride, last));
+            }
+            f(l, first);
+            i += stride;
         }
-        f(l, first);
     }
 }
 
@@ -242,7 +246,7 @@ struct Shared {
     double tab[128];
     union {
         u64 bins[kBins];
-        uint32_t count[kBins];
+        uint32_t count[kValues];
         u64 tile[kBins];
     };
     union {
@@ -313,18 +317,19 @@ __device__ __forceinline__ float block_sum(float v, Shared& sh) {
     return v;
 }
 
-// The place among four values a thread (in thread order) at which their running sum reaches `target` (> 0): sh.bin (kBins
+// The place among N values a thread (in thread order) at which their running sum reaches `target` (> 0): sh.bin (N * kThreads
 // where they do not), sh.above before it.  `extra` comes before the second half of the values.
-__device__ __forceinline__ void find_place(const u64 (&v)[kPer], u64 target, u64 extra, Shared& sh) {
+template <int N>
+__device__ __forceinline__ void find_place(const u64 (&v)[N], u64 target, u64 extra, Shared& sh) {
     u64 all, sum = 0;
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) sum += v[q];
+    for (int q = 0; q < N; ++q) sum += v[q];
     u64 upto = block_incl(sum, sh, &all) - sum + (threadIdx.x >= kThreads / 2 ? extra : 0);
-    if (threadIdx.x == 0) sh.bin = kBins, sh.above = all + extra;
+    if (threadIdx.x == 0) sh.bin = N * kThreads, sh.above = all + extra;
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        if (upto < target && target <= upto + v[q]) sh.bin = kPer * threadIdx.x + q, sh.above = upto;
+    for (int q = 0; q < N; ++q) {
+        if (upto < target && target <= upto + v[q]) sh.bin = N * threadIdx.x + q, sh.above = upto;
         upto += v[q];
     }
     __syncthreads();
@@ -569,7 +574,7 @@ __device__ __forceinline__ void append(u64 x, u64* list, uint32_t* n) {
 template <typename T>
 __device__ __forceinline__ float look_max(const T* row, uint32_t lo, uint32_t hi) {
     float top = -__builtin_inff();
-    each_element<8>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
+    each_element<4>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, l[e]);          // fmaxf drops NaN
     });
@@ -580,7 +585,7 @@ __device__ __forceinline__ float look_max(const T* row, uint32_t lo, uint32_t hi
 template <typename T>
 __device__ __forceinline__ void look_gather(const T* row, uint32_t lo, uint32_t hi, uint32_t klo, u64* list, uint32_t* n) {
     const float from = value_of(klo);                                // a candidate: NaN and -infinity fail the comparison
-    each_element<8>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t i) {
+    each_element<4>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t i) {
         if (fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= from) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -593,7 +598,7 @@ __device__ __forceinline__ void look_gather(const T* row, uint32_t lo, uint32_t 
 template <typename T, typename SH>
 __device__ __forceinline__ u64 look_bins(const T* row, uint32_t lo, uint32_t hi, const Row& r, SH& sh) {
     u64 sum = 0;
-    each_element<4>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
+    each_element<2>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
         u64 w[4];
         int bin[4];
 #pragma unroll
@@ -614,7 +619,7 @@ template <typename T, bool MASS>
 __device__ __forceinline__ void look_ranges(const T* row, uint32_t V, const Row& r, uint32_t klo, uint32_t khi, int shift, Shared& sh) {
     for (int q = 0; q < kPer; ++q) sh.bins[q * kThreads + threadIdx.x] = 0;
     __syncthreads();
-    each_element<4>(row, 0, V, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
+    each_element<2>(row, 0, V, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t key = key_of(l[e]);
@@ -627,24 +632,26 @@ __device__ __forceinline__ void look_ranges(const T* row, uint32_t V, const Row&
 
 // bfloat16 values with a counter have a place in descending order; the value of a place.
 __device__ __forceinline__ float value_of_place(uint32_t place) {
-    const uint32_t d = place < 2048 ? 2047 - place : place - 2048;
-    return __uint_as_float(((d + kFirstMag) << 16) | (place < 2048 ? 0u : 0x80000000u));
+    const uint32_t d = place < 4096 ? 4095 - place : place - 4096;
+    return __uint_as_float(((d + kFirstMag) << 16) | (place < 4096 ? 0u : 0x80000000u));
 }
 // Counts by value in sh.count, which the caller has cleared; candidates without a counter go to the list.  The counters lie
-// by magnitude, the negative ones behind: eight instructions an element, taken from the 16-bit halves as they are.
-__device__ __forceinline__ uint32_t place_of_counter(uint32_t c) { return c < 2048 ? 2047 - c : c; }       // in descending order
+// by magnitude, the negative ones behind.
+__device__ __forceinline__ uint32_t place_of_counter(uint32_t c) { return c < 4096 ? 4095 - c : c; }       // in descending order
 template <typename SH>
 __device__ __forceinline__ void look_values(const __bf16* row, uint32_t lo, uint32_t hi, SH& sh) {
-    each_element<8>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t i) {
+    each_element<4>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t i) {
+        bool out[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t u = __float_as_uint(l[e]), t = (u >> 16) - kFirstMag;      // sign in bit 15, 0 .. 2047 below it
-            if (!(t & 0x7800u)) {
-                const uint32_t at = (t & 0x7ffu) | ((t >> 4) & 0x800u);
-                atomicAdd(&sh.count[at], 1u);
-            } else if (candidate(l[e])) {
-                append(entry(key_of(l[e]), i + e), sh.list, &sh.n_list);
-            }
+            const uint32_t u = __float_as_uint(l[e]), d = (u & 0x7fffffffu) - (kFirstMag << 16);
+            out[e] = d >= 4096u << 16;
+            if (!out[e]) atomicAdd(&sh.count[(d >> 16) | ((u >> 19) & 4096u)], 1u);
+        }
+        if (out[0] || out[1] || out[2] || out[3]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (out[e] && candidate(l[e])) append(entry(key_of(l[e]), i + e), sh.list, &sh.n_list);
         }
     });
 }
@@ -815,12 +822,12 @@ __device__ __forceinline__ void border_by_bins(State& st, u64 of, Shared& sh) {
 
 // sh.count holds the counts by value, the list the n others: the border of top_k and top_p for look_tiles.
 __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st, uint32_t n, Shared& sh) {
-    uint32_t c[kPer];
-    float top = -__builtin_inff(), l[kPer];
+    uint32_t c[kPerValue];
+    float top = -__builtin_inff(), l[kPerValue];
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        c[q] = sh.count[place_of_counter(kPer * threadIdx.x + q)];
-        l[q] = value_of_place(kPer * threadIdx.x + q);
+    for (int q = 0; q < kPerValue; ++q) {
+        c[q] = sh.count[place_of_counter(kPerValue * threadIdx.x + q)];
+        l[q] = value_of_place(kPerValue * threadIdx.x + q);
         top = c[q] ? fmaxf(top, l[q]) : top;
     }
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) top = fmaxf(top, entry_value(sh.list[i]));
@@ -835,7 +842,7 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
     const float by = (float)(1.4426950408889634 * r.inv_t);
     float mass = 0.f;
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) mass += c[q] ? (float)c[q] * (l[q] == top ? 1.f : __builtin_amdgcn_exp2f((l[q] - top) * by)) : 0.f;
+    for (int q = 0; q < kPerValue; ++q) mass += c[q] ? (float)c[q] * (l[q] == top ? 1.f : __builtin_amdgcn_exp2f((l[q] - top) * by)) : 0.f;
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
         const float x = entry_value(sh.list[i]);
         mass += x == top ? 1.f : __builtin_amdgcn_exp2f((x - top) * by);
@@ -844,16 +851,16 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
     set_scale(r, top, fminf(mass * 1.01f + 1.f, (float)a.V));
     if (r.k == 0 && !(r.p < 1.0)) return;
     // in descending order: the list above the counters' range, the positive values, the list between, the negative, the rest
-    const float high = value_of_place(0), low = value_of_place(kBins - 1);
-    u64 w[kPer];
+    const float high = value_of_place(0), low = value_of_place(kValues - 1);
+    u64 w[kPerValue];
 #pragma unroll
-    for (int q = 0; q < kPer; ++q) w[q] = c[q] ? weight(r, l[q], sh.tab) : 0;
+    for (int q = 0; q < kPerValue; ++q) w[q] = c[q] ? weight(r, l[q], sh.tab) : 0;
     u64 of = 0;
 #pragma unroll 1
     for (int pass = r.k > 0 ? 0 : 1; pass < (r.p < 1.0 ? 2 : 1); ++pass) {           // by count, then by mass
-        u64 v[kPer], zone[4] = {0, 0, 0, 0};                         // the list's three, and the counters
+        u64 v[kPerValue], zone[4] = {0, 0, 0, 0};                         // the list's three, and the counters
 #pragma unroll
-        for (int q = 0; q < kPer; ++q) v[q] = pass ? w[q] * c[q] : c[q], zone[3] += v[q];
+        for (int q = 0; q < kPerValue; ++q) v[q] = pass ? w[q] * c[q] : c[q], zone[3] += v[q];
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
             const float x = entry_value(sh.list[i]);
             const u64 one = pass ? weight(r, x, sh.tab) : 1;
@@ -866,12 +873,12 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
         const u64 total = zone[0] + zone[1] + zone[2] + zone[3];
         if (pass == 0 && (u64)r.k >= total) continue;
         const u64 target = pass ? share_of(r.p, of ? of : total) : (u64)r.k;
-        uint32_t place = kBins;
+        uint32_t place = kValues;
         if (target > zone[0]) {
             find_place(v, target - zone[0], zone[1], sh);
             place = sh.bin;
         }
-        if (place < kBins) {
+        if (place < kValues) {
             const u64 need = target - zone[0] - sh.above;
             const float x = value_of_place(place);
             const u64 one = weight(r, x, sh.tab);
@@ -881,7 +888,7 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
             if (pass == 0) {
                 u64 above = 0;
 #pragma unroll
-                for (int q = 0; q < kPer; ++q) above += kPer * threadIdx.x + q < place ? w[q] * c[q] : 0;
+                for (int q = 0; q < kPerValue; ++q) above += kPerValue * threadIdx.x + q < place ? w[q] * c[q] : 0;
                 for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
                     const float y = entry_value(sh.list[i]);
                     above += y > x ? weight(r, y, sh.tab) : 0;
@@ -1036,7 +1043,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     const int64_t b = blockIdx.x;
     make_table(sh);
     if (threadIdx.x == 0) sh.n_list = 0;
-    for (int q = 0; q < kPer; ++q) sh.count[q * kThreads + threadIdx.x] = 0;
+    for (int q = 0; q < kPerValue; ++q) sh.count[q * kThreads + threadIdx.x] = 0;
     __syncthreads();
     const T* row = (const T*)a.logits + b * a.ld;
     if (a.V <= kSmall) {                                             // the list, whatever the settings
@@ -1076,7 +1083,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
 // Between the kernels a row's state lies in the workspace.  The looks run on gridDim.x segments of whole tiles a row, the
 // steps between them on one block a row.
 struct RowSpace {
-    u64 bins[kBins];                // the first half of it: counts of bfloat16 values
+    u64 bins[kBins];                // or the kValues counts of bfloat16 values
     u64 tile[kBins];
     u64 list[kBins];
     uint32_t ties[kBins];
@@ -1113,7 +1120,7 @@ __global__ __launch_bounds__(kThreads, 8) void split_max_kernel(SampleArgs a, Ro
 
 __global__ __launch_bounds__(kThreads) void split_clear_kernel(RowSpace* ws) {
     RowSpace& w = ws[blockIdx.x];
-    for (int i = threadIdx.x; i < kBins / 2; i += kThreads) w.bins[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) w.bins[i] = 0;
     if (threadIdx.x == 0) w.n_list = 0;
 }
 
@@ -1129,7 +1136,7 @@ __device__ __forceinline__ void to_row_list(SH& sh, RowSpace& w) {
 
 // bfloat16: the counts of the values.
 struct SharedValues {
-    uint32_t count[kBins];
+    uint32_t count[kValues];
     u64 list[kBins];
     uint32_t n_list, base;
 };
@@ -1137,13 +1144,13 @@ __global__ __launch_bounds__(kThreads, 8) void split_values_kernel(SampleArgs a,
     __shared__ SharedValues sh;
     RowSpace& w = ws[blockIdx.y];
     const Segment s = segment(a);
-    for (int q = 0; q < kPer; ++q) sh.count[q * kThreads + threadIdx.x] = 0;
+    for (int q = 0; q < kPerValue; ++q) sh.count[q * kThreads + threadIdx.x] = 0;
     if (threadIdx.x == 0) sh.n_list = 0;
     __syncthreads();
     if (s.t0 < s.t1) look_values((const __bf16*)a.logits + blockIdx.y * a.ld, s.lo, s.hi, sh);
     __syncthreads();
     uint32_t* count = reinterpret_cast<uint32_t*>(w.bins);
-    for (int q = 0; q < kPer; ++q) {
+    for (int q = 0; q < kPerValue; ++q) {
         const uint32_t c = sh.count[q * kThreads + threadIdx.x];
         if (c) atomicAdd(&count[q * kThreads + threadIdx.x], c);
     }
@@ -1168,7 +1175,7 @@ __global__ __launch_bounds__(kThreads) void split_plan_kernel(SampleArgs a, RowS
         const uint32_t n = w.n_list;
         if (n <= kBins) {
             const uint32_t* count = reinterpret_cast<const uint32_t*>(w.bins);
-            for (int q = 0; q < kPer; ++q) sh.count[q * kThreads + threadIdx.x] = count[q * kThreads + threadIdx.x];
+            for (int q = 0; q < kPerValue; ++q) sh.count[q * kThreads + threadIdx.x] = count[q * kThreads + threadIdx.x];
             for (uint32_t i = threadIdx.x; i < n; i += kThreads) sh.list[i] = w.list[i];
             __syncthreads();
             border_by_values(a, st, n, sh);
