@@ -659,12 +659,12 @@ __device__ __forceinline__ void look_values(const __bf16* row, uint32_t lo, uint
 // Tile by tile of [t0, t1): the weights above khi, and of the elements from klo to khi the count (TIES) or the entries in the
 // list.  Values are compared, not keys: two comparisons an element.  Where few are kept, a wave lines them up in its
 // part of `queue` (128 entries) and takes their weights 64 at a time.
-template <typename T>
+template <bool TIES, typename T>
 __device__ __forceinline__ void look_tiles(const SampleArgs& a, const T* row, const State& st, uint32_t t0, uint32_t t1, const double* tab,
                                            float* queue, u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);      // one value: the loops below are the wave's
     const Row r = st.r;
-    const bool count = st.ties;
     const float above = st.khi < kLowestKey ? -__builtin_inff() : value_of(st.khi);
     const float from = st.klo <= st.khi ? value_of(st.klo) : __builtin_inff();      // with no border: nothing from `from` to `above`
     float* line = queue + 128 * wave;
@@ -685,7 +685,7 @@ __device__ __forceinline__ void look_tiles(const SampleArgs& a, const T* row, co
             if (border[0] | border[1] | border[2] | border[3]) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (count) n += __popcll(border[e]);
+                    if (TIES) n += __popcll(border[e]);
                     else if ((border[e] >> lane) & 1) append(entry(key_of(l[e]), i + e), list, n_list);
                 }
             }
@@ -717,7 +717,7 @@ __device__ __forceinline__ void look_tiles(const SampleArgs& a, const T* row, co
         w = wave_incl(w);
         if (lane == 63) {
             tile[t] = w;
-            if (count) ties[t] = n;
+            if (TIES) ties[t] = n;
         }
     }
 }
@@ -957,7 +957,9 @@ __device__ __forceinline__ void look_tiles_alone(const SampleArgs& a, const T* r
     __syncthreads();
     if (threadIdx.x == 0) sh.n_list = 0;
     __syncthreads();
-    look_tiles(a, row, st, 0, (a.V + a.tile - 1) / a.tile, sh.tab, sh.queue, sh.tile, sh.ties, sh.list, &sh.n_list);
+    const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
+    if (st.ties) look_tiles<true>(a, row, st, 0, tiles, sh.tab, sh.queue, sh.tile, sh.ties, sh.list, &sh.n_list);
+    else look_tiles<false>(a, row, st, 0, tiles, sh.tab, sh.queue, sh.tile, sh.ties, sh.list, &sh.n_list);
     __syncthreads();
 }
 
@@ -1239,7 +1241,8 @@ __global__ __launch_bounds__(kThreads, 8) void split_look_kernel(SampleArgs a, R
     make_table(sh);
     if (mode == kTiles) {
         __syncthreads();
-        look_tiles(a, row, w.st, s.t0, s.t1, sh.tab, sh.queue, w.tile, w.ties, w.list, &w.n_list);
+        if (w.st.ties) look_tiles<true>(a, row, w.st, s.t0, s.t1, sh.tab, sh.queue, w.tile, w.ties, w.list, &w.n_list);
+        else look_tiles<false>(a, row, w.st, s.t0, s.t1, sh.tab, sh.queue, w.tile, w.ties, w.list, &w.n_list);
         return;
     }
     if (mode == kGather) {
