@@ -42,6 +42,7 @@ constexpr int kValues = 2 * 4096, kPerValue = kValues / kThreads;
 
 typedef unsigned long long u64;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 struct SampleArgs {
     const void* logits;
@@ -77,6 +78,7 @@ struct Raw<float> {
     f32x4 v;
     __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(&v, p, 16); }
     __device__ __forceinline__ float get(int e) const { return v[e]; }
+    __device__ __forceinline__ void drop(int e) { v[e] = __builtin_nanf(""); }
 };
 template <>
 struct Raw<__bf16> {
@@ -86,13 +88,14 @@ struct Raw<__bf16> {
         const uint32_t w = e < 2 ? v.x : v.y;
         return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
     }
+    __device__ __forceinline__ void drop(int e) { (e < 2 ? v.x : v.y) |= e & 1 ? 0x7fff0000u : 0x7fffu; }
 };
 
-// f(four values, index of the first) for the elements of [lo, hi), hi >= 4, by `threads` threads (all of them take part in
-// every step; values outside are NaN), DEPTH steps' loads in flight.  The loop is unrolled over these: a load's register must
-// not be moved while it is awaited.
+// f(Raw of four elements, index of the first) for the elements of [lo, hi), hi >= 4, by `threads` threads (all of them take
+// part in every step; elements outside are NaN), DEPTH steps' loads in flight.  The loop is unrolled over these: a load's
+// register must not be moved while it is awaited.
 template <int DEPTH, typename T, typename F>
-__device__ __forceinline__ void each_element(const T* row, uint32_t lo, uint32_t hi, int thread, int threads, F f) {
+__device__ __forceinline__ void each_raw(const T* row, uint32_t lo, uint32_t hi, int thread, int threads, F f) {
     const uint32_t stride = threads * 4, steps = (hi - lo + stride - 1) / stride, last = hi - 4;
     uint32_t i = lo + thread * 4;
     Raw<T> ahead[DEPTH];
@@ -103,19 +106,30 @@ __device__ __forceinline__ void each_element(const T* row, uint32_t lo, uint32_t
 #pragma unroll
         for (int q = 0; q < DEPTH; ++q) {
             if (n + q >= steps) break;
-            float l[4] = {ahead[q].get(0), ahead[q].get(1), ahead[q].get(2), ahead[q].get(3)};
             uint32_t first = i;
             if (n + q + 1 == steps) {               // past the end: the row's last four, without what came before
                 first = std::min(i, last);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) l[e] = first + e >= i ? l[e] : __builtin_nanf("");
+                for (int e = 0; e < 4; ++e)
+                    if (first + e < i) ahead[q].drop(e);
+                f(ahead[q], first);
             } else {
+                const Raw<T> x = ahead[q];
                 ahead[q].load(row + std::min(i + DEPTH * stride, last));
+                f(x, first);
             }
-            f(l, first);
             i += stride;
         }
     }
+}
+
+// f(four values, index of the first)
+template <int DEPTH, typename T, typename F>
+__device__ __forceinline__ void each_element(const T* row, uint32_t lo, uint32_t hi, int thread, int threads, F f) {
+    each_raw<DEPTH>(row, lo, hi, thread, threads, [&](const Raw<T>& x, uint32_t first) {
+        const float l[4] = {x.get(0), x.get(1), x.get(2), x.get(3)};
+        f(l, first);
+    });
 }
 
 // ------------------------------------------------------------------------------- weights
@@ -242,6 +256,7 @@ struct State {
     u64 need;                       // elements of the border key, or units of the border bin's mass
 };
 
+constexpr int kLine = 96;            // fours in a wave's queue: a full load of 64 and as many as may come too many
 struct Shared {
     double tab[128];
     union {
@@ -254,7 +269,7 @@ struct Shared {
         float group[kBins];
     };
     uint32_t ties[kBins];
-    float queue[kWaves * 128];
+    f32x4 queue[kWaves * kLine];
     State st;
     u64 wsum[kWaves], wsums[4][kWaves];
     float wmax[kWaves];
@@ -636,85 +651,98 @@ __device__ __forceinline__ float value_of_place(uint32_t place) {
     return __uint_as_float(((d + kFirstMag) << 16) | (place < 4096 ? 0u : 0x80000000u));
 }
 // Counts by value in sh.count, which the caller has cleared; candidates without a counter go to the list.  The counters lie
-// by magnitude, the negative ones behind.
+// by magnitude, the negative ones behind; two elements are worked on in a register.
 __device__ __forceinline__ uint32_t place_of_counter(uint32_t c) { return c < 4096 ? 4095 - c : c; }       // in descending order
 template <typename SH>
 __device__ __forceinline__ void look_values(const __bf16* row, uint32_t lo, uint32_t hi, SH& sh) {
-    each_element<4>(row, lo, hi, threadIdx.x, kThreads, [&](const float(&l)[4], uint32_t i) {
-        bool out[4];
+    char* const count = reinterpret_cast<char*>(sh.count);
+    each_raw<4>(row, lo, hi, threadIdx.x, kThreads, [&](const Raw<__bf16>& x, uint32_t i) {
+        uint32_t d[2], at[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t w = h ? x.v.y : x.v.x;
+            const u16x2 m = __builtin_bit_cast(u16x2, w & 0x7fff7fffu) - (unsigned short)kFirstMag;
+            d[h] = __builtin_bit_cast(uint32_t, m);
+            at[h] = (d[h] << 2) | ((w >> 1) & 0x40004000u);          // bytes; no carry where both have a counter
+        }
+        if (!((d[0] | d[1]) & 0xf000f000u)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                atomicAdd(reinterpret_cast<uint32_t*>(count + (at[h] & 0xffffu)), 1u);
+                atomicAdd(reinterpret_cast<uint32_t*>(count + (at[h] >> 16)), 1u);
+            }
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t u = __float_as_uint(l[e]), d = (u & 0x7fffffffu) - (kFirstMag << 16);
-            out[e] = d >= 4096u << 16;
-            if (!out[e]) atomicAdd(&sh.count[(d >> 16) | ((u >> 19) & 4096u)], 1u);
-        }
-        if (out[0] || out[1] || out[2] || out[3]) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (out[e] && candidate(l[e])) append(entry(key_of(l[e]), i + e), sh.list, &sh.n_list);
+            const float l = x.get(e);
+            const uint32_t one = e & 1 ? d[e / 2] >> 16 : d[e / 2] & 0xffffu;
+            if (one < 4096) atomicAdd(&sh.count[one | (l < 0 ? 4096 : 0)], 1u);
+            else if (candidate(l)) append(entry(key_of(l), i + e), sh.list, &sh.n_list);
         }
     });
 }
 
 // Tile by tile of [t0, t1): the weights above khi, and of the elements from klo to khi the count (TIES) or the entries in the
-// list.  Values are compared, not keys: two comparisons an element.  Where few are kept, a wave lines them up in its
-// part of `queue` (128 entries) and takes their weights 64 at a time.
+// list.  Values are compared, not keys, four at once.  Where few are kept, a wave lines up the fours that hold one in its
+// part of `queue` and takes their weights 64 fours at a time.
 template <bool TIES, typename T>
 __device__ __forceinline__ void look_tiles(const SampleArgs& a, const T* row, const State& st, uint32_t t0, uint32_t t1, const double* tab,
-                                           float* queue, u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
+                                           f32x4* queue, u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);      // one value: the loops below are the wave's
     const Row r = st.r;
     const float above = st.khi < kLowestKey ? -__builtin_inff() : value_of(st.khi);
     const float from = st.klo <= st.khi ? value_of(st.klo) : __builtin_inff();      // with no border: nothing from `from` to `above`
-    float* line = queue + 128 * wave;
+    f32x4* line = queue + kLine * wave;
     for (uint32_t t = t0 + wave; t < t1; t += kWaves) {
         u64 w = 0;
         uint32_t n = 0, queued = 0;
-        auto flush = [&](uint32_t m) {                               // the first m (at most 64) of the line
-            const u64 x = weight(r, lane < m ? line[lane] : -__builtin_inff(), tab);
-            w += x;
+        auto add = [&](const float* l) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w += weight(r, l[e] > above ? l[e] : -__builtin_inff(), tab);
         };
         each_element<4>(row, t * a.tile, std::min(a.V, (t + 1) * a.tile), lane, 64, [&](const float(&l)[4], uint32_t i) {
-            u64 kept[4], border[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                kept[e] = __ballot(l[e] > above);
-                border[e] = __ballot(l[e] >= from) & ~kept[e];
-            }
-            if (border[0] | border[1] | border[2] | border[3]) {
+            const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));          // fmaxf drops NaN
+            const bool some = top > above;
+            const u64 kept = __ballot(some);
+            if (__ballot(top >= from)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if (TIES) n += __popcll(border[e]);
-                    else if ((border[e] >> lane) & 1) append(entry(key_of(l[e]), i + e), list, n_list);
+                    const bool border = l[e] >= from && !(l[e] > above);
+                    if (TIES) n += border;
+                    else if (border) append(entry(key_of(l[e]), i + e), list, n_list);
                 }
             }
-            if (!(kept[0] | kept[1] | kept[2] | kept[3])) return;
-            if (__popcll(kept[0]) + __popcll(kept[1]) + __popcll(kept[2]) + __popcll(kept[3]) > 64) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w += weight(r, l[e] > above ? l[e] : -__builtin_inff(), tab);
-                return;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (l[e] > above) line[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(kept[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)kept[e], 0))] = l[e];
-                queued += __popcll(kept[e]);
-            }
+            if (!kept) return;
+            const uint32_t more = __popcll(kept);
+            if (more > kLine - 64) return add(l);
+            if (some) line[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(kept >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)kept, 0))] = {l[0], l[1], l[2], l[3]};
+            queued += more;
+            if (queued < 64) return;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            if (queued >= 64) {
-                const float rest = line[64 + lane];
-                flush(64);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                line[lane] = rest;
-                queued -= 64;
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-            }
+            const f32x4 x = line[lane], rest = line[64 + (lane & (kLine - 65))];
+            const float four[4] = {x[0], x[1], x[2], x[3]};
+            add(four);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (lane < kLine - 64) line[lane] = rest;
+            queued -= 64;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
         });
-        if (queued) flush(queued);
+        if (queued) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const f32x4 x = line[lane];
+            const float four[4] = {x[0], x[1], x[2], x[3]};
+            if (lane < queued) add(four);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
         w = wave_incl(w);
+        if (TIES) n = (uint32_t)wave_incl((u64)n);
         if (lane == 63) {
             tile[t] = w;
             if (TIES) ties[t] = n;
@@ -1225,7 +1253,7 @@ struct SharedLook {
         u64 bins[kBins];
         u64 list[kBins];
     };
-    float queue[kWaves * 128];
+    f32x4 queue[kWaves * kLine];
     u64 mass;
     uint32_t n_list, base;
 };
