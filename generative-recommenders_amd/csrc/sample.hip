@@ -106,18 +106,17 @@ __device__ __forceinline__ void each_raw(const T* row, uint32_t lo, uint32_t hi,
 #pragma unroll
         for (int q = 0; q < DEPTH; ++q) {
             if (n + q >= steps) break;
+            Raw<T> x = ahead[q];
             uint32_t first = i;
             if (n + q + 1 == steps) {               // past the end: the row's last four, without what came before
                 first = std::min(i, last);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (first + e < i) ahead[q].drop(e);
-                f(ahead[q], first);
+                    if (first + e < i) x.drop(e);
             } else {
-                const Raw<T> x = ahead[q];
                 ahead[q].load(row + std::min(i + DEPTH * stride, last));
-                f(x, first);
             }
+            f(x, first);
             i += stride;
         }
     }
@@ -257,6 +256,10 @@ struct State {
 };
 
 constexpr int kLine = 96;            // fours in a wave's queue: a full load of 64 and as many as may come too many
+struct Line {
+    f32x4 four[kLine];
+    uint32_t t[kLine];
+};
 struct Shared {
     double tab[128];
     union {
@@ -269,7 +272,7 @@ struct Shared {
         float group[kBins];
     };
     uint32_t ties[kBins];
-    f32x4 queue[kWaves * kLine];
+    Line queue[kWaves];
     State st;
     u64 wsum[kWaves], wsums[4][kWaves];
     float wmax[kWaves];
@@ -683,71 +686,88 @@ __device__ __forceinline__ void look_values(const __bf16* row, uint32_t lo, uint
     });
 }
 
-// Tile by tile of [t0, t1): the weights above khi, and of the elements from klo to khi the count (TIES) or the entries in the
-// list.  Values are compared, not keys, four at once.  Where few are kept, a wave lines up the fours that hold one in its
-// part of `queue` and takes their weights 64 fours at a time.
+// Tile by tile of [t0, t1), each wave its share: adds the weights above khi to tile[t - t0], which the caller has cleared, and
+// of the elements from klo to khi the count to ties[t] (TIES) or the entries to the list.  Values are compared, not keys, four
+// at once.  Where few are kept, a wave lines up the fours that hold one and takes their weights 64 fours at a time: a weight
+// is some 40 instructions, and few of a step's 64 fours hold one.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 template <bool TIES, typename T>
 __device__ __forceinline__ void look_tiles(const SampleArgs& a, const T* row, const State& st, uint32_t t0, uint32_t t1, const double* tab,
-                                           f32x4* queue, u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
+                                           Line* queue, u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);      // one value: the loops below are the wave's
     const Row r = st.r;
     const float above = st.khi < kLowestKey ? -__builtin_inff() : value_of(st.khi);
     const float from = st.klo <= st.khi ? value_of(st.klo) : __builtin_inff();      // with no border: nothing from `from` to `above`
-    f32x4* line = queue + kLine * wave;
-    for (uint32_t t = t0 + wave; t < t1; t += kWaves) {
-        u64 w = 0;
-        uint32_t n = 0, queued = 0;
-        auto add = [&](const float* l) {
+    Line& line = queue[wave];
+    const uint32_t per = (t1 - t0 + kWaves - 1) / kWaves, per_tile = a.tile / 256;
+    uint32_t t = t0 + wave * per, left = per_tile;                   // steps left of tile t
+    if (t >= t1) return;
+    const uint32_t hi = std::min(a.V, std::min(t + per, t1) * a.tile);
+    u64 w = 0;
+    uint32_t n = 0, queued = 0;
+    auto take = [&](uint32_t m) {                                    // the first m (at most 64) fours of the line
+        wave_sync();
+        const f32x4 x = line.four[lane];
+        const uint32_t at = line.t[lane] - t0;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bits |= x[e] > above ? 1 << e : 0;
+        if (lane >= m) bits = 0;
+#pragma unroll 1
+        while (__any(bits != 0)) {                                   // mostly once or twice
+            if (bits) {
+                const float l = bits & 1 ? x[0] : bits & 2 ? x[1] : bits & 4 ? x[2] : x[3];
+                atomicAdd(&tile[at], weight(r, l, tab));
+                bits &= bits - 1;
+            }
+        }
+        wave_sync();
+    };
+    auto store = [&] {                                               // the end of tile t
+        if (__any(w != 0)) {
+            const u64 all = wave_incl(w);
+            if (lane == 63) atomicAdd(&tile[t - t0], all);
+        }
+        if (TIES && lane == 0) ties[t] = n;
+        w = 0, n = 0, ++t, left = per_tile;
+    };
+    each_element<4>(row, t * a.tile, hi, lane, 64, [&](const float(&l)[4], uint32_t i) {
+        const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));          // fmaxf drops NaN
+        const bool some = top > above;
+        const u64 kept = __ballot(some);
+        if (__any(top >= from)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool border = l[e] >= from && !(l[e] > above);
+                if (TIES) n += __popcll(__ballot(border));
+                else if (border) append(entry(key_of(l[e]), i + e), list, n_list);
+            }
+        }
+        const uint32_t more = __popcll(kept);
+        if (more > kLine - 64) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) w += weight(r, l[e] > above ? l[e] : -__builtin_inff(), tab);
-        };
-        each_element<4>(row, t * a.tile, std::min(a.V, (t + 1) * a.tile), lane, 64, [&](const float(&l)[4], uint32_t i) {
-            const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));          // fmaxf drops NaN
-            const bool some = top > above;
-            const u64 kept = __ballot(some);
-            if (__ballot(top >= from)) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool border = l[e] >= from && !(l[e] > above);
-                    if (TIES) n += border;
-                    else if (border) append(entry(key_of(l[e]), i + e), list, n_list);
-                }
-            }
-            if (!kept) return;
-            const uint32_t more = __popcll(kept);
-            if (more > kLine - 64) return add(l);
-            if (some) line[queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(kept >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)kept, 0))] = {l[0], l[1], l[2], l[3]};
+        } else if (more) {
+            const uint32_t at = queued + __builtin_amdgcn_mbcnt_hi((uint32_t)(kept >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)kept, 0));
+            if (some) line.four[at] = {l[0], l[1], l[2], l[3]}, line.t[at] = t;
             queued += more;
-            if (queued < 64) return;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            const f32x4 x = line[lane], rest = line[64 + (lane & (kLine - 65))];
-            const float four[4] = {x[0], x[1], x[2], x[3]};
-            add(four);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if (lane < kLine - 64) line[lane] = rest;
-            queued -= 64;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        });
-        if (queued) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            const f32x4 x = line[lane];
-            const float four[4] = {x[0], x[1], x[2], x[3]};
-            if (lane < queued) add(four);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            if (queued >= 64) {
+                take(64);
+                const f32x4 rest = line.four[64 + (lane & (kLine - 65))];
+                const uint32_t rest_t = line.t[64 + (lane & (kLine - 65))];
+                wave_sync();
+                if (lane < kLine - 64) line.four[lane] = rest, line.t[lane] = rest_t;
+                queued -= 64;
+            }
         }
-        w = wave_incl(w);
-        if (TIES) n = (uint32_t)wave_incl((u64)n);
-        if (lane == 63) {
-            tile[t] = w;
-            if (TIES) ties[t] = n;
-        }
-    }
+        if (--left == 0) store();
+    });
+    if (left < per_tile) store();                                    // the row's end
+    if (queued) take(queued);
 }
 
 // ------------------------------------------------------------------------------- borders
@@ -984,6 +1004,7 @@ template <typename T>
 __device__ __forceinline__ void look_tiles_alone(const SampleArgs& a, const T* row, const State& st, Shared& sh) {
     __syncthreads();
     if (threadIdx.x == 0) sh.n_list = 0;
+    for (int q = 0; q < kPer; ++q) sh.tile[q * kThreads + threadIdx.x] = 0;
     __syncthreads();
     const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
     if (st.ties) look_tiles<true>(a, row, st, 0, tiles, sh.tab, sh.queue, sh.tile, sh.ties, sh.list, &sh.n_list);
@@ -1253,7 +1274,7 @@ struct SharedLook {
         u64 bins[kBins];
         u64 list[kBins];
     };
-    f32x4 queue[kWaves * kLine];
+    Line queue[kWaves];
     u64 mass;
     uint32_t n_list, base;
 };
@@ -1268,9 +1289,12 @@ __global__ __launch_bounds__(kThreads, 8) void split_look_kernel(SampleArgs a, R
     if (s.t0 >= s.t1) return;
     make_table(sh);
     if (mode == kTiles) {
+        for (uint32_t t = threadIdx.x; t < s.t1 - s.t0; t += kThreads) sh.bins[t] = 0;
         __syncthreads();
-        if (w.st.ties) look_tiles<true>(a, row, w.st, s.t0, s.t1, sh.tab, sh.queue, w.tile, w.ties, w.list, &w.n_list);
-        else look_tiles<false>(a, row, w.st, s.t0, s.t1, sh.tab, sh.queue, w.tile, w.ties, w.list, &w.n_list);
+        if (w.st.ties) look_tiles<true>(a, row, w.st, s.t0, s.t1, sh.tab, sh.queue, sh.bins, w.ties, w.list, &w.n_list);
+        else look_tiles<false>(a, row, w.st, s.t0, s.t1, sh.tab, sh.queue, sh.bins, w.ties, w.list, &w.n_list);
+        __syncthreads();
+        for (uint32_t t = threadIdx.x; t < s.t1 - s.t0; t += kThreads) w.tile[s.t0 + t] = sh.bins[t];
         return;
     }
     if (mode == kGather) {
