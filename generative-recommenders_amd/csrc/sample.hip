@@ -92,8 +92,9 @@ struct Raw<__bf16> {
 };
 
 // f(Raw of four elements, index of the first) for the elements of [lo, hi), hi >= 4, by `threads` threads (all of them take
-// part in every step; elements outside are NaN), DEPTH steps' loads in flight.  The loop is unrolled over these: a load's
-// register must not be moved while it is awaited.
+// part in every step; elements outside are NaN), DEPTH steps' loads in flight.  The loop is unrolled over these, since a load's
+// register must not be moved while it is awaited, and every step has its load, also past the end (of the last four): the
+// compiler counts the loads to wait for, and one that may be missing makes it wait for all.
 template <int DEPTH, typename T, typename F>
 __device__ __forceinline__ void each_raw(const T* row, uint32_t lo, uint32_t hi, int thread, int threads, F f) {
     const uint32_t stride = threads * 4, steps = (hi - lo + stride - 1) / stride, last = hi - 4;
@@ -107,14 +108,13 @@ __device__ __forceinline__ void each_raw(const T* row, uint32_t lo, uint32_t hi,
         for (int q = 0; q < DEPTH; ++q) {
             if (n + q >= steps) break;
             Raw<T> x = ahead[q];
+            ahead[q].load(row + std::min(i + DEPTH * stride, last));
             uint32_t first = i;
             if (n + q + 1 == steps) {               // past the end: the row's last four, without what came before
                 first = std::min(i, last);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (first + e < i) x.drop(e);
-            } else {
-                ahead[q].load(row + std::min(i + DEPTH * stride, last));
             }
             f(x, first);
             i += stride;
