@@ -902,7 +902,10 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
     const float high = value_of_place(0), low = value_of_place(kValues - 1);
     u64 w[kPerValue];
 #pragma unroll
-    for (int q = 0; q < kPerValue; ++q) w[q] = c[q] ? weight(r, l[q], sh.tab) : 0;
+    for (int q = 0; q < kPerValue; ++q) {                            // many waves have no value that occurs
+        w[q] = 0;
+        if (__any(c[q] != 0)) w[q] = c[q] ? weight(r, l[q], sh.tab) : 0;
+    }
     u64 of = 0;
 #pragma unroll 1
     for (int pass = r.k > 0 ? 0 : 1; pass < (r.p < 1.0 ? 2 : 1); ++pass) {           // by count, then by mass
@@ -917,7 +920,13 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
             zone[1] += at == 1 ? one : 0;
             zone[2] += at == 2 ? one : 0;
         }
-        block_sums(zone, sh);
+        if (n) {
+            block_sums(zone, sh);
+        } else {
+            u64 all[1] = {zone[3]};
+            block_sums(all, sh);
+            zone[3] = all[0];
+        }
         const u64 total = zone[0] + zone[1] + zone[2] + zone[3];
         if (pass == 0 && (u64)r.k >= total) continue;
         const u64 target = pass ? share_of(r.p, of ? of : total) : (u64)r.k;
