@@ -1377,12 +1377,14 @@ __global__ __launch_bounds__(kThreads) void split_border_kernel(SampleArgs a, Ro
 // Blocks over which a row is cut; 1: not cut.  One block's time grows with the row, a cut row costs four to six launches, and
 // from some 64 rows on the rows fill the card by themselves.  Measured, us, one block a row / cut (spread 3, T = 1):
 //                         top_k 50 fp32   top_p 0.9 fp32   no border fp32   top_p 0.9 bf16
-//    1 x    32,768         15 /  20         28 /  32         17 / 17          24 / 27
-//    1 x    65,536         19 /  21         41 /  32         26 / 17          33 / 27
-//    1 x   131,072         25 /  24         70 /  33         46 / 17          52 / 28
-//    1 x 1,000,000        114 /  26        443 /  43        307 / 22         298 / 34
-//   64 x   131,072         27 /  28         72 /  66         47 / 32          53 / 39
-//  128 x   131,072         36 /  43         79 /  92         54 / 48          53 / 49
+//    1 x    32,768         14 /  14         26 /  31         15 / 16          21 / 27
+//    1 x    65,536         15 /  15         38 /  42         23 / 16          28 / 27
+//    1 x   131,072         18 /  19         61 /  43         39 / 17          40 / 27
+//    1 x 1,000,000         67 /  22        374 /  42        254 / 21         206 / 31
+//   64 x   131,072         20 /  25         63 /  64         40 / 30          41 / 38
+//  128 x   131,072         29 /  39         72 /  93         47 / 46          42 / 44
+// Where every row leads to a list by a small top_k, one block looks at it but twice: 1 x 262,144 27 / 20, 32 x 262,144 27 / 25,
+// 64 x 500,000 54 / 57.
 int splits(int64_t B, int64_t V) {
     const int64_t c = std::min<int64_t>(std::min<int64_t>(512 / B, V / 4096), kMaxSplit);
     return V >= 1 << 16 && c >= 8 ? (int)c : 1;
@@ -1430,7 +1432,7 @@ extern "C" int hmx_sample_logits(const void* logits, int64_t ld, int64_t B, int6
     if (workspace_bytes < hmx_sample_logits_workspace_bytes(B, V) || (C > 1 && !workspace)) return HMX_EWORKSPACE;
     SampleArgs a = {logits, ld, (uint32_t)V, u, u_f64 != 0, (int)draws, temperature, top_p, min_p, top_k, temperature_all,
                     top_p_all, min_p_all, top_k_all, ids, probs, (uint32_t)(hmx_ceil_div(V, (int64_t)kBins * kTile) * kTile)};
-    if (C > 1 && (bf16 || V >= 1 << 17 || !listed(a, kThreads))) {
+    if (C > 1 && (bf16 || !listed(a, kThreads) || (V >= 1 << 18 && B <= 32))) {
         if (bf16) launch_split<__bf16>(a, B, C, (RowSpace*)workspace, (hipStream_t)stream);
         else launch_split<float>(a, B, C, (RowSpace*)workspace, (hipStream_t)stream);
     } else if (bf16) {
