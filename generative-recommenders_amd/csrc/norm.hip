@@ -5,6 +5,10 @@
 // squares and the scaling), backward reads s, dy, ds and writes dx once.  LPR lanes share a row; a lane owns NV vectors
 // of VEC consecutive columns (16 bytes when the rows allow it, single columns otherwise), so LPR * NV * VEC >= d.
 // Sums are fp32 in a fixed order (lane, then a butterfly over the lanes, then over the waves): no atomics.
+// Measured, us (a copy of 1 GiB: 5.1 TB/s): 102,400 x 64 fp32 forward 22.6 (4.7 TB/s), backward 19.2 + 4.2 for the column sums
+// (its operands partly from cache); 16,384 x 4096 bf16 forward 92 (5.8 TB/s), backward 112 + 6 (4.8 TB/s, 17 MB of partials
+// included: 4 blocks a compute unit keep them few); 8191 x 1000 fp32 into 8 bits 22.9 (4.7 TB/s); 1024 x 64: 3.3 and 5.7,
+// 1 x 4096 into 8 bits 4.3: the launch.
 #include "hmx_common.h"
 
 #include <algorithm>

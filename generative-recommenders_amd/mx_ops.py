@@ -67,7 +67,8 @@ def _dequantize(what, bits, codes, scales, d, dtype):
 
 
 def dequantize_mx8(codes, scales, d=None, dtype=torch.bfloat16):
-    """The values that mx8 codes stand for, (..., d); d None: all dp of them.  bfloat16 holds each exactly."""
+    """The values that mx8 codes stand for, (..., d); d None: all dp of them.  float32 holds each exactly, bfloat16 from
+    2^-126 up (it rounds to multiples of 2^-133 below)."""
     return _dequantize("dequantize_mx8", 8, codes, scales, d, dtype)
 
 
@@ -76,17 +77,23 @@ def dequantize_mx4(codes, scales, d=None, dtype=torch.bfloat16):
     return _dequantize("dequantize_mx4", 4, codes, scales, d, dtype)
 
 
-def quantize_mx4(table):
+def quantize_mx4(table, out=None):
     """table (..., d) float32 or bfloat16 -> (codes uint8 (..., dp / 2), scales uint8 (..., dp / 32)).  Run it again
-    after the table's weights changed."""
+    after the table's weights changed; out (codes, scales): it is written there, for captured graphs that read it."""
     device = _one_device("quantize_mx4", table)
     if table.dtype not in (torch.float32, torch.bfloat16) or table.dim() < 1 or table.shape[-1] < 1:
         raise hmx.HmxError(f"quantize_mx4: a float32 or bfloat16 table of rows, got {table.dtype} {tuple(table.shape)}")
     t2 = _rows(table)
     n, d = t2.shape
     dp = padded(d)
-    codes = torch.empty(*table.shape[:-1], dp // 2, dtype=torch.uint8, device=device)
-    scales = torch.empty(*table.shape[:-1], dp // BLOCK, dtype=torch.uint8, device=device)
+    shapes = (*table.shape[:-1], dp // 2), (*table.shape[:-1], dp // BLOCK)
+    if out is None:
+        codes, scales = (torch.empty(s, dtype=torch.uint8, device=device) for s in shapes)
+    else:
+        codes, scales = out
+        if any(t.shape != s or t.dtype != torch.uint8 or t.device != device or not t.is_contiguous()
+               for t, s in zip(out, shapes)):
+            raise hmx.HmxError(f"quantize_mx4: out is contiguous uint8 {shapes[0]} and {shapes[1]} on {device}")
     _launch("hmx_mx4_quantize", device, t2.data_ptr(), t2.stride(0), n, d, int(table.dtype == torch.bfloat16),
             codes.data_ptr(), scales.data_ptr())
     return codes, scales
@@ -98,8 +105,8 @@ _X_KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
 def linear_mx4(x, codes, scales, x_scales=None, out_dtype=torch.float32):
     """out (..., N) = x (..., K) times the transposed mx4 table (codes (N, dp / 2), scales (N, dp / 32)), dp = padded(K).
 
-    x is float32 (all 24 bits take part), bfloat16, or mx8 codes (..., dp) with x_scales (..., dp / 32); sums are
-    float32, out is float32 or bfloat16.  Made for few rows of x: the scores of a batch of users over an item table, a
+    x is float32 (all 24 bits take part), bfloat16, or mx8 codes (..., dp) with x_scales (..., dp / 32); bits of x below
+    2^-133 are left out.  Sums are float32, out is float32 or bfloat16; no gradient.  Made for few rows of x: the scores of a batch of users over an item table, a
     layer for single tokens.  More rows re-read the table once per 32 (layers) or 16 (K <= 128)."""
     device, n, blocks, codes, scales = _checked("linear_mx4", codes, scales, torch.uint8, BLOCK // 2)
     if scales.dim() != 2:

@@ -346,13 +346,17 @@ class SampledRetriever:
     def __init__(self, table, id_offset=0, score_bytes=1 << 30):
         self.id_offset = int(id_offset)
         self.score_bytes = int(score_bytes)
+        self.codes = None
         self.refresh(table)
 
     def refresh(self, table):
-        """Call after the table's weights changed (quantises it again)."""
+        """Call after the table's weights changed: quantises it again, into the same memory where its shape is the same (a
+        captured sample() then reads the new weights)."""
         from . import mx_ops
+        same = self.codes is not None and self.codes.device == table.device and \
+            (self.codes.shape[0], self.dim) == tuple(table.shape)
         self.dim = table.shape[1]
-        self.codes, self.scales = mx_ops.quantize_mx4(table.detach())
+        self.codes, self.scales = mx_ops.quantize_mx4(table.detach(), (self.codes, self.scales) if same else None)
 
     def scores(self, states, norm_scale=None, residual=None, eps=1e-6):
         """(n, d) states -> (n, items) fp32 scores.  norm_scale (d,): the states are first added to `residual` (where given)

@@ -674,13 +674,13 @@ int hmx_add_rmsnorm_mx8(const void* x, int64_t ldx, const void* residual, int64_
 
 /* A (n, d) table (fp32, or bfloat16 where bf16 = 1; row stride ld in elements) in mx4: codes (n, dp / 2), scales
  * (n, dp / 32), and the values that mx4 (bits = 4) or mx8 (bits = 8) codes stand for, (n, d) fp32 or bfloat16: exact in
- * both, infinite from 2^128 on. */
+ * both, but infinite from 2^128 on and, as bfloat16, rounded to multiples of 2^-133 below 2^-126. */
 int hmx_mx4_quantize(const void* table, int64_t ld, int64_t n, int64_t d, int bf16, void* codes, void* scales, void* stream);
 int hmx_mx_dequantize(const void* codes, const void* scales, int64_t n, int64_t d, int bits, int bf16, void* out, void* stream);
 
 /* out (M, N) = x (M, K) * W^T for an mx4 table W (N, K).  x_kind 0: fp32 rows of stride ldx (elements), all 24 bits of a
- * value take part; 1: bfloat16; 2: mx8 codes (ldx = dp) with x_scales (M, dp / 32).  Sums in fp32; out contiguous, fp32 or
- * bfloat16 (out_bf16 = 1). */
+ * value take part; 1: bfloat16; 2: mx8 codes (ldx = dp) with x_scales (M, dp / 32).  Bits of x below 2^-133 are left out
+ * (mx8: rounded).  Sums in fp32; out contiguous, fp32 or bfloat16 (out_bf16 = 1). */
 size_t hmx_linear_mx4_workspace_bytes(int x_kind, int64_t M, int64_t K);
 int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, int x_kind, int64_t M, const void* codes, const void* scales,
                    int64_t N, int64_t K, int out_bf16, void* out, void* workspace, size_t workspace_bytes, void* stream);

@@ -264,3 +264,33 @@ def test_graph_and_stream():
         again = mx_ops.linear_mx4(xs, codes, scales)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("k", [64, 200])
+def test_smallest_x(k):
+    # one product a row, a power of two times 1.5: exact wherever x's own bits are taken
+    w = torch.zeros(70, k, device=DEV)
+    w[:, 3] = 1.5 * 2.0 ** 120
+    codes, scales = mx_ops.quantize_mx4(w)
+    exps = [-100, -126, -127, -130, -133, -134, -149]
+    x = torch.zeros(len(exps), k, device=DEV)
+    x[:, 3] = torch.tensor([2.0 ** e for e in exps], dtype=torch.float64).float().to(DEV)
+    want = torch.tensor([1.5 * 2.0 ** (120 + e) if e >= -133 else 0.0 for e in exps])
+    for xs in (x, x.bfloat16()):
+        got = mx_ops.linear_mx4(xs, codes, scales).cpu()
+        assert torch.equal(got, want[:, None].expand_as(got))
+
+
+def test_quantize_into_given_memory():
+    first, second = torch.randn(300, 50, device=DEV), torch.randn(300, 50, device=DEV)
+    out = mx_ops.quantize_mx4(first)
+    at = [t.data_ptr() for t in out]
+    again = mx_ops.quantize_mx4(second, out=out)
+    want = mx_ops.quantize_mx4(second)
+    assert [t.data_ptr() for t in again] == at
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    codes, scales = out
+    for bad in ((codes[:299], scales), (codes, scales[:, :1]), (codes.to(torch.int8), scales), (codes.cpu(), scales),
+                (torch.empty(300, 64, dtype=torch.uint8, device=DEV)[:, ::2], scales)):
+        with pytest.raises(hmx.HmxError):
+            mx_ops.quantize_mx4(second, out=bad)

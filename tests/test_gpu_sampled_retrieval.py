@@ -109,6 +109,24 @@ def test_graph_of_the_whole_path():
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
 
 
+def test_refresh_reaches_a_captured_graph():
+    table, h, res, scale, u = setup(n=3, items=70001, seed=8)
+    rt = SampledRetriever(table)
+    settings = dict(temperature=0.8, top_p=0.9, norm_scale=scale)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rt.sample(h, u, **settings)
+    for k in range(3):
+        new = table.roll(1000 * (k + 1), 0) * (1 + k)
+        rt.refresh(new)
+        graph.replay()
+        want = SampledRetriever(new).sample(h, u, **settings)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    rt.refresh(table[:500])                      # another shape: memory of its own
+    assert rt.sample(h, u)[0].max() < 500
+
+
 def test_refusals():
     table, h, res, scale, u = setup()
     rt = SampledRetriever(table)
