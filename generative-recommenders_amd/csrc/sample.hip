@@ -6,7 +6,8 @@
 //
 // Weights are fp64 (z exactly as far as fp64 goes, exp by table and polynomial, 1e-15) turned into integers w * 2^s, with s
 // the largest scale at which the row's mass is sure to fit 62 bits (51 at most): integer sums do not depend on their order,
-// so LDS and global atomics, any split of a row and any number of waves give the same set and the same draw.
+// so LDS and global atomics and any number of waves give the same set and the same draw on every run.  (How a row is worked on,
+// by its length and the number of rows, sets the bound on its mass and so the scale: one rounding of a weight.)
 //
 // What bounds it: at four cycles a wave an instruction per element costs 0.9 us for 33.5 M elements on the whole card, so the
 // few instructions that every element meets come first, the 25 of a weight where they can be spared:
