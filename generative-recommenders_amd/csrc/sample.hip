@@ -479,10 +479,50 @@ __device__ __forceinline__ void draw_nothing(const SampleArgs& a, int64_t b) {
     for (int q = threadIdx.x; q < a.draws; q += kThreads) a.ids[b * a.draws + q] = -1, a.probs[b * a.draws + q] = 0.f;
 }
 
-// The draws by the tiles' sums (sh.tile): the kept elements are the entries from `last` on that pass min_p.  One wave a draw
-// finds the tile by running sums, then the element, 1024 elements' loads at once.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The draw of a tile whose kept elements are few, by the wave, from the list's first n entries: false where they are more than
+// 64.  `before`: the weights of earlier tiles.
+__device__ __forceinline__ bool draw_from_entries(const SampleArgs& a, const Row& r, uint32_t n, uint32_t from, uint32_t end, u64 before,
+                                                  u64 want, int64_t at, u64 total, u64* hits, const Shared& sh) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t m = 0;
+    wave_sync();
+    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+        const u64 x = sh.list[std::min(i0 + lane, n - 1)];
+        const uint32_t i = ~(uint32_t)x;
+        const bool in = i0 + lane < n && i >= from && i < end;
+        const u64 all = __ballot(in);
+        if (!all) continue;
+        const uint32_t place = m + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+        if (in && place < 64) hits[place] = x;
+        m += __popcll(all);
+    }
+    wave_sync();
+    if (m > 64) return false;
+    const u64 x = hits[lane];
+    const uint32_t own = ~(uint32_t)x;
+    const float l = entry_value(x);
+    const u64 w = lane < m && passes(r, l) ? weight(r, l, sh.tab) : 0;
+    u64 sum = before;                                                // of the elements before the lane's own
+    for (uint32_t q = 0; q < m; ++q) {
+        const uint32_t other = __builtin_amdgcn_readlane((int)own, q);
+        const u64 one = lane64(w, q);
+        sum += other < own ? one : 0;
+    }
+    const bool hit = w != 0 && sum <= want && want < sum + w;
+    if (hit) put_draw(a, r, at, own, l, total, sh.tab);
+    return __any(hit);
+}
+
+// The draws by the tiles' sums (sh.tile): the kept elements are the entries from `last` on that pass min_p; where `listed` is
+// not 0, they are among the list's first `listed` entries.  One wave a draw finds the tile by running sums, then the element:
+// among the list's entries where a tile has few of them (no read of the row: 7 -> 3 us), or with 1024 elements' loads at once.
 template <typename T>
-__device__ __forceinline__ void draw_by_tiles(const SampleArgs& a, const T* row, const Row& r, u64 last, int64_t b, Shared& sh) {
+__device__ __forceinline__ void draw_by_tiles(const SampleArgs& a, const T* row, const Row& r, u64 last, uint32_t listed, int64_t b, Shared& sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t tiles = (a.V + a.tile - 1) / a.tile;
     u64 w[kPer], sum = 0, total;
@@ -504,7 +544,9 @@ __device__ __forceinline__ void draw_by_tiles(const SampleArgs& a, const T* row,
         const uint32_t lo = 64 * part + __ffsll((long long)__ballot(sh.tile[64 * part + lane] > want)) - 1;
         u64 before = lo ? sh.tile[lo - 1] : 0;
         const uint32_t end = std::min(a.V, (lo + 1) * a.tile);
-        bool found = false;
+        bool found = listed && listed <= 16 * tiles &&
+                     draw_from_entries(a, r, listed, lo * a.tile, end, before, want, b * a.draws + q, total,
+                                       reinterpret_cast<u64*>(sh.queue[wave].four), sh);
 #pragma unroll 1
         for (uint32_t i0 = lo * a.tile; i0 < end && !found; i0 += kTile) {
             float l[4][4];
@@ -583,7 +625,7 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, const T* row
     for (int q = 0; q < kPer; ++q) sh.tile[q * kThreads + threadIdx.x] = 0;
     __syncthreads();
     list_to_tiles(a, r, keep, sh);
-    draw_by_tiles(a, row, r, last, b, sh);
+    draw_by_tiles(a, row, r, last, keep, b, sh);
 }
 
 // ------------------------------------------------------------------------------- looks at the elements
@@ -694,10 +736,6 @@ __device__ __forceinline__ void look_values(const __bf16* row, uint32_t lo, uint
 // of the elements from klo to khi the count to ties[t] (TIES) or the entries to the list.  Values are compared, not keys, four
 // at once.  Where few are kept, a wave lines up the fours that hold one and takes their weights 64 fours at a time: a weight
 // is some 40 instructions, and few of a step's 64 fours hold one.
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
 template <bool TIES, typename T>
 __device__ __forceinline__ void look_tiles(const SampleArgs& a, const T* row, const State& st, uint32_t t0, uint32_t t1, const double* tab,
                                            Line* queue, u64* tile, uint32_t* ties, u64* list, uint32_t* n_list) {
@@ -1008,7 +1046,7 @@ __device__ __forceinline__ bool draw_from_tiles(const SampleArgs& a, const T* ro
             __syncthreads();
         }
     }
-    draw_by_tiles(a, row, r, last, b, sh);
+    draw_by_tiles(a, row, r, last, 0, b, sh);
     return true;
 }
 
