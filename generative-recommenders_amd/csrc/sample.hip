@@ -340,13 +340,15 @@ __device__ __forceinline__ float block_sum(float v, Shared& sh) {
 }
 
 // The place among N values a thread (in thread order) at which their running sum reaches `target` (> 0): sh.bin (N * kThreads
-// where they do not), sh.above before it.  `extra` comes before the second half of the values.
-template <int N>
-__device__ __forceinline__ void find_place(const u64 (&v)[N], u64 target, u64 extra, Shared& sh) {
+// where they do not), sh.above before it.  `extra` comes before the second half of the values.  SHARE: the target is a share of
+// the sum.
+template <bool SHARE = false, int N>
+__device__ __forceinline__ void find_place(const u64 (&v)[N], u64 target, u64 extra, Shared& sh, double share = 1.0) {
     u64 all, sum = 0;
 #pragma unroll
     for (int q = 0; q < N; ++q) sum += v[q];
     u64 upto = block_incl(sum, sh, &all) - sum + (threadIdx.x >= kThreads / 2 ? extra : 0);
+    if (SHARE) target = share_of(share, all);
     if (threadIdx.x == 0) sh.bin = N * kThreads, sh.above = all + extra;
     __syncthreads();
 #pragma unroll
@@ -454,7 +456,8 @@ __device__ __forceinline__ void sort_by_ranges(uint32_t n, uint32_t klo, uint32_
     __syncthreads();
 }
 
-// The place in the list's first n entries (sorted) at which their running mass reaches `target`.
+// The place in the list's first n entries (sorted) at which their running mass reaches `target`, or (SHARE) top_p of theirs.
+template <bool SHARE>
 __device__ __forceinline__ uint32_t place_of_mass(const Row& r, uint32_t n, u64 target, Shared& sh) {
     u64 v[kPer];
 #pragma unroll
@@ -462,7 +465,7 @@ __device__ __forceinline__ uint32_t place_of_mass(const Row& r, uint32_t n, u64 
         const uint32_t i = kPer * threadIdx.x + q;
         v[q] = i < n ? weight(r, entry_value(sh.list[i]), sh.tab) : 0;
     }
-    find_place(v, target, 0, sh);
+    find_place<SHARE>(v, target, 0, sh, r.p);
     return n ? std::min(sh.bin, n - 1) : 0;
 }
 
@@ -613,12 +616,7 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, const T* row
     if ((r.k > 0 && r.k < n) || r.p < 1.0) {
         sort_by_ranges(n, klo, r.top, sh);
         if (r.k > 0 && r.k < n) keep = (uint32_t)r.k;
-        if (r.p < 1.0) {
-            u64 total[1] = {0};
-            for (uint32_t i = threadIdx.x; i < keep; i += kThreads) total[0] += weight(r, entry_value(sh.list[i]), sh.tab);
-            block_sums(total, sh);
-            keep = place_of_mass(r, keep, share_of(r.p, total[0]), sh) + 1;
-        }
+        if (r.p < 1.0) keep = place_of_mass<true>(r, keep, 0, sh) + 1;
         last = sh.list[keep - 1];
     }
     __syncthreads();
@@ -853,23 +851,30 @@ __device__ __forceinline__ void fold_min_p(State& st) {
     if (lo >= st.khi) st.klo = lo + 1, st.khi = lo, st.ties = 1, st.need = 0;
 }
 
-// The lowest key that the gather needs: of the bin in which the k-th largest of the groups' maxima lies (0: below the bins).
+// A key that k elements reach, and few more: the least of the groups' maxima in the bin of the k-th largest of them (0: below
+// the bins).
 __device__ __forceinline__ uint32_t key_by_maxima(const Row& r, int groups, Shared& sh) {
     for (int q = 0; q < kPer; ++q) sh.count[q * kThreads + threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.at = ~0u;
     __syncthreads();
-    for (int g = threadIdx.x; g < groups; g += kThreads) {
+    auto bin = [&](int g) {
         const float m = sh.group[g];
-        const int b = candidate(m) ? bin_of(r, m) : kBins;
-        if (b < kBins) atomicAdd(&sh.count[b], 1u);
+        return candidate(m) ? bin_of(r, m) : kBins;
+    };
+    for (int g = threadIdx.x; g < groups; g += kThreads) {
+        const int at = bin(g);
+        if (at < kBins) atomicAdd(&sh.count[at], 1u);
     }
     __syncthreads();
     u64 v[kPer];
 #pragma unroll
     for (int q = 0; q < kPer; ++q) v[q] = sh.count[kPer * threadIdx.x + q];
     find_place(v, (u64)r.k, 0, sh);
-    uint32_t first = 0, last;
-    if (sh.bin < kBins) keys_of_bin(r, sh.bin, &first, &last);
-    return first;
+    if (sh.bin >= kBins) return 0;
+    for (int g = threadIdx.x; g < groups; g += kThreads)
+        if (bin(g) == (int)sh.bin) atomicMin(&sh.at, key_of(sh.group[g]));
+    __syncthreads();
+    return sh.at;
 }
 
 // Narrows the keys klo to khi, which hold the border, to its own key; *need becomes the number of that key's elements that
@@ -1040,7 +1045,7 @@ __device__ __forceinline__ bool draw_from_tiles(const SampleArgs& a, const T* ro
             const uint32_t n = sh.n_list;
             if (n > kBins) return false;
             sort_list<true>(n, sh.list);
-            const uint32_t place = place_of_mass(r, n, st.need, sh);
+            const uint32_t place = place_of_mass<false>(r, n, st.need, sh);
             list_to_tiles(a, r, place + 1, sh);
             last = sh.list[place];
             __syncthreads();
