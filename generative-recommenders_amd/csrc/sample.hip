@@ -24,8 +24,8 @@
 // One block does a row on its own; few long rows are cut into segments for the looks at all elements, with one block a row
 // between them.
 // Measured, us: 256 x 131,072 bf16 47 in one launch: the count of values 9.5, the border from 8192 counters 8, the tiles 14, the
-// draws 6 (67 MB once at 5.1 TB/s: 13); 4 x 4,000,001 fp32, top_k 1000 and 16 draws 49: maxima 12, plan 8, gather 13, list and
-// draws 16; 1 x 50,000 fp32, top_k 50: 14.
+// draws 6 (67 MB once at 5.1 TB/s: 13); 4 x 4,000,001 fp32, top_k 1000 and 16 draws 44: maxima 12, plan 6, gather 13, list and
+// draws 13; 1 x 50,000 fp32, top_k 50: 12.
 #include "hmx_common.h"
 
 #include <algorithm>
@@ -1424,14 +1424,13 @@ __global__ __launch_bounds__(kThreads) void split_border_kernel(SampleArgs a, Ro
 // Blocks over which a row is cut; 1: not cut.  One block's time grows with the row, a cut row costs four to six launches, and
 // from some 64 rows on the rows fill the card by themselves.  Measured, us, one block a row / cut (spread 3, T = 1):
 //                         top_k 50 fp32   top_p 0.9 fp32   no border fp32   top_p 0.9 bf16
-//    1 x    32,768         14 /  14         26 /  31         15 / 16          21 / 27
-//    1 x    65,536         15 /  15         38 /  42         23 / 16          28 / 27
-//    1 x   131,072         18 /  19         61 /  43         39 / 17          40 / 27
-//    1 x 1,000,000         67 /  22        374 /  42        254 / 21         206 / 31
-//   64 x   131,072         20 /  25         63 /  64         40 / 30          41 / 38
-//  128 x   131,072         29 /  39         72 /  93         47 / 46          42 / 44
-// Where every row leads to a list by a small top_k, one block looks at it but twice: 1 x 262,144 27 / 20, 32 x 262,144 27 / 25,
-// 64 x 500,000 54 / 57.
+//    1 x    32,768         11 /  16         26 /  31         15 / 16          21 / 27
+//    1 x   131,072         16 /  17         60 /  32         39 / 17          39 / 27
+//    1 x 1,000,000         65 /  19        371 /  41        254 / 21         205 / 31
+//   64 x   131,072         18 /  22         63 /  64         40 / 30          41 / 38
+//  128 x   131,072         27 /  36         72 /  93         47 / 45          41 / 45
+// Where every row leads to a list by a small top_k, one block looks at it but twice: 1 x 262,144 24 / 17, 32 x 262,144 25 / 21,
+// 64 x 500,000 52 / 53.
 int splits(int64_t B, int64_t V) {
     const int64_t c = std::min<int64_t>(std::min<int64_t>(512 / B, V / 4096), kMaxSplit);
     return V >= 1 << 16 && c >= 8 ? (int)c : 1;
@@ -1476,7 +1475,9 @@ extern "C" int hmx_sample_logits(const void* logits, int64_t ld, int64_t B, int6
     if (B == 0 || draws == 0) return HMX_OK;
     if (!logits || !u || !ids || !probs) return HMX_EINVAL;
     const int C = splits(B, V);
-    if (workspace_bytes < hmx_sample_logits_workspace_bytes(B, V) || (C > 1 && !workspace)) return HMX_EWORKSPACE;
+    if (workspace_bytes < hmx_sample_logits_workspace_bytes(B, V) ||
+        (C > 1 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)))
+        return HMX_EWORKSPACE;
     SampleArgs a = {logits, ld, (uint32_t)V, u, u_f64 != 0, (int)draws, temperature, top_p, min_p, top_k, temperature_all,
                     top_p_all, min_p_all, top_k_all, ids, probs, (uint32_t)(hmx_ceil_div(V, (int64_t)kBins * kTile) * kTile)};
     if (C > 1 && (bf16 || !listed(a, kThreads) || (V >= 1 << 18 && B <= 32))) {
