@@ -239,6 +239,16 @@ __device__ __forceinline__ bf16x8 decode_bf16(uint32_t word, float scale) {
     return __builtin_bit_cast(bf16x8, w);
 }
 
+// Eight mx8 codes (two words) and their scale: what convertvector makes of the values, bit for bit.
+__device__ __forceinline__ bf16x8 decode_bf16(uint32_t lo, uint32_t hi, float scale) {
+    u32x4 w;
+    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    return __builtin_bit_cast(bf16x8, w);
+}
+
 __device__ __forceinline__ bf16x8 zero_if(bool z, bf16x8 v) {
     u32x4 w = __builtin_bit_cast(u32x4, v);
 #pragma unroll
@@ -415,14 +425,31 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(LinearArgs a, int chun
     packed[t] = __builtin_bit_cast(u32x4, v);
 }
 
+// mx8 rows stay in 8 bits, half of what bf16 would have the second launch read: per tile and chunk, half h of a lane's block
+// and lane, 16 codes, and behind all of these the scale byte of each lane.
+__global__ __launch_bounds__(256) void linear_pack_mx8_kernel(LinearArgs a, int chunks, int64_t total, u32x4* __restrict__ packed) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;          // (unit, half, lane)
+    if (t >= total) return;
+    const int lane = (int)(t & 63), h = (int)(t >> 6) & 1;
+    const int64_t unit = t >> 7;
+    const int chunk = (int)(unit % chunks), m = (int)(unit / chunks) * 16 + (lane & 15);
+    if (m >= a.M) return;                                               // lanes that the second launch leaves out
+    const int b = 8 * (chunk >> 1) + 2 * (lane >> 4) + (chunk & 1);
+    const int64_t block = (int64_t)m * a.nblk + b;
+    packed[t] = b < a.nblk ? ((const u32x4*)a.x)[2 * block + h] : u32x4{0, 0, 0, 0};
+    if (h == 0) reinterpret_cast<uint8_t*>(packed + total)[unit * 64 + lane] = b < a.nblk ? a.xs[block] : 127;
+}
+
 // What lanes past the end of a row load in place of codes and scales.
 __device__ const u32x4 kZeros = {};
 
 // The second: W waves a block, KW of them share 16 RT rows of the table and split its K (256 columns in turn, two chunks of
 // 128 of which a lane has two neighbouring blocks: a wave reads whole 128-byte lines); their sums meet in LDS and are added in
 // wave order.  The next chunk is in flight while one is multiplied.  TERMS: operand rows of a row of x.
-template <int TERMS, int W, int MT, int RT, typename OUT>
-__global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const u32x4* __restrict__ packed, int KW) {
+template <int XK, int W, int MT, int RT, typename OUT>
+__global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const u32x4* __restrict__ packed,
+                                                             const uint8_t* __restrict__ packed_scales, int KW) {
+    constexpr int TERMS = planes<XK>(), XV = XK == kXMx8 ? 2 : 4;    // vectors of x to a lane's block
     constexpr int NE = RT * MT * 4, ROWS = TERMS == 3 ? 5 : 16;      // rows of x to a tile
     __shared__ float red[W][NE][64];
     const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4, wave = threadIdx.x >> 6;
@@ -447,7 +474,8 @@ __global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const
     // blocks in step would all wait for it
     const int pairs = chunks / 2, mine = 2 * ((pairs - kw + KW - 1) / KW), turn = (int)(blockIdx.x * 37u % (unsigned)pairs);
     struct Chunk {
-        u32x4 w[RT], x[MT][4];
+        u32x4 w[RT], x[MT][XV];
+        uint8_t xs[MT];
     };
     uint32_t sc[RT];                                                 // both chunks' scales, the second's in the upper byte
     const int64_t all = a.N * a.nblk;
@@ -462,12 +490,15 @@ __global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const
         for (int r = 0; r < RT; ++r) t.w[r] = *(past ? &kZeros : a.codes + row_at[r] + b);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const u32x4* p = packed + (((int64_t)(blockIdx.y * MT + m) * chunks + chunk) * 4) * 64 + lane;
+            const int64_t unit = (int64_t)(blockIdx.y * MT + m) * chunks + chunk;
+            const u32x4* p = packed + unit * (64 * XV) + lane;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < XV; ++i) {
                 t.x[m][i] = u32x4{0, 0, 0, 0};
                 if (used[m] && !past) t.x[m][i] = p[64 * i];
             }
+            t.xs[m] = 127;
+            if (XK == kXMx8 && used[m] && !past) t.xs[m] = packed_scales[unit * 64 + lane];
         }
     };
     auto fetch_scales = [&](int n, uint32_t (&sd)[RT]) {             // of the pair that the n-th chunk begins
@@ -486,14 +517,20 @@ __global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const
 #pragma unroll
         for (int r = 0; r < RT; ++r) s[r] = scale_value((sc[r] >> (8 * half)) & 255u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            bf16x8 xv[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                if constexpr (XK == kXMx8) xv[m] = decode_bf16(t.x[m][i / 2][2 * (i & 1)], t.x[m][i / 2][2 * (i & 1) + 1], scale_value(t.xs[m]));
+                else xv[m] = __builtin_bit_cast(bf16x8, t.x[m][i]);
+            }
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 const bf16x8 wv = decode_bf16(t.w[r][i], s[r]);
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    acc[r][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.x[m][i]), wv, acc[r][m], 0, 0, 0);
+                for (int m = 0; m < MT; ++m) acc[r][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv[m], wv, acc[r][m], 0, 0, 0);
             }
+        }
     };
     if (n0 < a.N && mine > 0) {
         Chunk even, odd;
@@ -563,14 +600,17 @@ void launch_linear(const LinearArgs& a, u32x4* packed, hipStream_t st) {
         return;
     }
     const int chunks = 2 * (int)hmx_ceil_div(a.nblk, 8), tiles = operand_tiles(XK, a.M);
-    const int64_t total = (int64_t)tiles * chunks * 256;
-    hipLaunchKernelGGL(linear_pack_kernel<XK>, dim3((unsigned)hmx_ceil_div(total, 256)), dim3(256), 0, st, a, chunks, total, packed);
+    const int64_t total = (int64_t)tiles * chunks * (XK == kXMx8 ? 128 : 256);
+    const dim3 pack_grid((unsigned)hmx_ceil_div(total, 256));
+    if constexpr (XK == kXMx8) hipLaunchKernelGGL(linear_pack_mx8_kernel, pack_grid, dim3(256), 0, st, a, chunks, total, packed);
+    else hipLaunchKernelGGL(linear_pack_kernel<XK>, pack_grid, dim3(256), 0, st, a, chunks, total, packed);
+    const uint8_t* packed_scales = reinterpret_cast<const uint8_t*>(packed + total);
     int kw = kWavesLong;
     while (kw > 1 && chunks < 4 * kw) kw /= 2;
 #define LONG(MT, RT)                                                                                                      \
-    hipLaunchKernelGGL((linear_long_kernel<planes<XK>(), kWavesLong, MT, RT, OUT>),                                       \
+    hipLaunchKernelGGL((linear_long_kernel<XK, kWavesLong, MT, RT, OUT>),                                                  \
                        dim3((unsigned)hmx_ceil_div(a.N, 16 * RT * (kWavesLong / kw)), (unsigned)hmx_ceil_div(tiles, MT)), \
-                       dim3(64 * kWavesLong), 0, st, a, packed, kw)
+                       dim3(64 * kWavesLong), 0, st, a, packed, packed_scales, kw)
     // two tiles of x a wave share what decoding W costs, two of W what loading x does; one of W where two would leave compute
     // units without a block (32 x 4096 x 4096 mx8: 9.0 us against 10.4)
     const bool wide = hmx_ceil_div(a.N, 32 * (kWavesLong / kw)) >= 256;
