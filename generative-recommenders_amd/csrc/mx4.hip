@@ -404,12 +404,12 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
     }
 }
 
-// Longer rows go in two launches.  The first lays x out as the second one's lanes take it: per tile of 16 operand rows and
+// Longer rows, more than 8 of them, go in two launches.  The first lays x out as the second one's lanes take it: per tile of 16 operand rows and
 // 128 columns, step i and lane, the eight bf16 values of one MFMA operand.  An fp32 row is three operand rows (its terms; five
 // rows of x to a tile), any other one.  Read as it lies, x cost more than W: rows of a power of two of bytes lie in one
-// memory channel and one set of the cache, and every block decodes all of x (32 x 8192 x 8192 mx8: 22 us, this way 15 and 3).  What
-// bounds the second: every block reads all of x from L2 (134 MB there; with x at one address it takes 6 us less, with W at
-// one address 5), and what a launch's waves need to start.
+// memory channel and one set of the cache, and every block decodes all of x (32 x 8192 x 8192 mx8: 22 us, this way 14 and 3).  What
+// bounds the second: every block reads all of x from L2 (as bfloat16 134 MB there: with x at one address it took 6 us less,
+// with W at one address 5; as mx8 half of that), and what a launch's waves need to start.
 template <int XK>
 __global__ __launch_bounds__(256) void linear_pack_kernel(LinearArgs a, int chunks, int64_t total, u32x4* __restrict__ packed) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -445,8 +445,9 @@ __device__ const u32x4 kZeros = {};
 
 // The second: W waves a block, KW of them share 16 RT rows of the table and split its K (256 columns in turn, two chunks of
 // 128 of which a lane has two neighbouring blocks: a wave reads whole 128-byte lines); their sums meet in LDS and are added in
-// wave order.  The next chunk is in flight while one is multiplied.  TERMS: operand rows of a row of x.
-template <int XK, int W, int MT, int RT, typename OUT>
+// wave order.  The next chunk is in flight while one is multiplied.  TERMS: operand rows of a row of x; PACKED: x comes from the
+// first launch.
+template <int XK, bool PACKED, int W, int MT, int RT, typename OUT>
 __global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const u32x4* __restrict__ packed,
                                                              const uint8_t* __restrict__ packed_scales, int KW) {
     constexpr int TERMS = planes<XK>(), XV = XK == kXMx8 ? 2 : 4;    // vectors of x to a lane's block
@@ -491,14 +492,16 @@ __global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const int64_t unit = (int64_t)(blockIdx.y * MT + m) * chunks + chunk;
-            const u32x4* p = packed + unit * (64 * XV) + lane;
+            const int row = (int)(blockIdx.y * MT + m) * 16 + c;     // not PACKED: of x itself
+            const u32x4* p = PACKED ? packed + unit * (64 * XV) + lane
+                                    : (const u32x4*)a.x + (XK == kXMx8 ? (int64_t)row * a.nblk * XV : row * (a.ldx / 8)) + (int64_t)b * XV;
 #pragma unroll
             for (int i = 0; i < XV; ++i) {
                 t.x[m][i] = u32x4{0, 0, 0, 0};
-                if (used[m] && !past) t.x[m][i] = p[64 * i];
+                if (used[m] && !past) t.x[m][i] = p[(PACKED ? 64 : 1) * i];
             }
             t.xs[m] = 127;
-            if (XK == kXMx8 && used[m] && !past) t.xs[m] = packed_scales[unit * 64 + lane];
+            if (XK == kXMx8 && used[m] && !past) t.xs[m] = PACKED ? packed_scales[unit * 64 + lane] : a.xs[(int64_t)row * a.nblk + b];
         }
     };
     auto fetch_scales = [&](int n, uint32_t (&sd)[RT]) {             // of the pair that the n-th chunk begins
@@ -577,6 +580,7 @@ __global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 constexpr int kWavesLong = 8;
+constexpr int kDirect = 8;
 
 // Tiles of 16 operand rows that M rows of x make for linear_long_kernel.
 int operand_tiles(int x_kind, int64_t M) { return (int)hmx_ceil_div(M, x_kind == kXF32 ? 5 : 16); }
@@ -600,22 +604,31 @@ void launch_linear(const LinearArgs& a, u32x4* packed, hipStream_t st) {
         return;
     }
     const int chunks = 2 * (int)hmx_ceil_div(a.nblk, 8), tiles = operand_tiles(XK, a.M);
-    const int64_t total = (int64_t)tiles * chunks * (XK == kXMx8 ? 128 : 256);
-    const dim3 pack_grid((unsigned)hmx_ceil_div(total, 256));
-    if constexpr (XK == kXMx8) hipLaunchKernelGGL(linear_pack_mx8_kernel, pack_grid, dim3(256), 0, st, a, chunks, total, packed);
-    else hipLaunchKernelGGL(linear_pack_kernel<XK>, pack_grid, dim3(256), 0, st, a, chunks, total, packed);
-    const uint8_t* packed_scales = reinterpret_cast<const uint8_t*>(packed + total);
     int kw = kWavesLong;
     while (kw > 1 && chunks < 4 * kw) kw /= 2;
-#define LONG(MT, RT)                                                                                                      \
-    hipLaunchKernelGGL((linear_long_kernel<XK, kWavesLong, MT, RT, OUT>),                                                  \
+#define LONG(PACKED, MT, RT)                                                                                              \
+    hipLaunchKernelGGL((linear_long_kernel<XK, PACKED, kWavesLong, MT, RT, OUT>),                                          \
                        dim3((unsigned)hmx_ceil_div(a.N, 16 * RT * (kWavesLong / kw)), (unsigned)hmx_ceil_div(tiles, MT)), \
                        dim3(64 * kWavesLong), 0, st, a, packed, packed_scales, kw)
     // two tiles of x a wave share what decoding W costs, two of W what loading x does; one of W where two would leave compute
-    // units without a block (32 x 4096 x 4096 mx8: 9.0 us against 10.4)
+    // units without a block (32 x 4096 x 4096 mx8: 8.5 us against 10.0; 32 x 8192 x 8192, which has enough: 17.9 against 16.0)
     const bool wide = hmx_ceil_div(a.N, 32 * (kWavesLong / kw)) >= 256;
-    if (tiles == 1) { if (wide) LONG(1, 2); else LONG(1, 1); }
-    else { if (wide) LONG(2, 2); else LONG(2, 1); }
+    const int64_t total = (int64_t)tiles * chunks * (XK == kXMx8 ? 128 : 256);
+    const uint8_t* packed_scales = reinterpret_cast<const uint8_t*>(packed + total);
+    // few rows are read as they lie (fp32 has to be cut, a bf16 row has to have whole blocks): one launch, and the rows share
+    // few enough cache lines.  As they lie / packed: 1 x 8192 x 8192 bf16 10.7 / 13.3 us, 8 rows 13.4 / 13.8, 16 rows 18.6 / 14.5;
+    // 1 x 1000 x 5024 4.4 / 6.8; 8 x 8192 x 8192 mx8 12.1 / 13.1, 16 rows 14.3 / 13.3
+    if constexpr (XK != kXF32) {
+        if (a.M <= kDirect && (XK == kXMx8 || ((a.M == 1 || a.ldx % 8 == 0) && a.K % 32 == 0 && aligned(a.x, 16)))) {
+            if (wide) LONG(false, 1, 2); else LONG(false, 1, 1);
+            return;
+        }
+    }
+    const dim3 pack_grid((unsigned)hmx_ceil_div(total, 256));
+    if constexpr (XK == kXMx8) hipLaunchKernelGGL(linear_pack_mx8_kernel, pack_grid, dim3(256), 0, st, a, chunks, total, packed);
+    else hipLaunchKernelGGL(linear_pack_kernel<XK>, pack_grid, dim3(256), 0, st, a, chunks, total, packed);
+    if (tiles == 1) { if (wide) LONG(true, 1, 2); else LONG(true, 1, 1); }
+    else { if (wide) LONG(true, 2, 2); else LONG(true, 2, 1); }
 #undef LONG
 }
 

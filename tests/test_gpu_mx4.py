@@ -294,3 +294,23 @@ def test_quantize_into_given_memory():
                 (torch.empty(300, 64, dtype=torch.uint8, device=DEV)[:, ::2], scales)):
         with pytest.raises(hmx.HmxError):
             mx_ops.quantize_mx4(second, out=bad)
+
+
+@pytest.mark.parametrize("n,k", [(70, 160), (1000, 1024), (8200, 2048)])
+def test_few_long_rows_read_as_they_lie_or_packed(n, k):
+    # the same products in the same order whichever way x comes
+    codes, scales = mx_ops.quantize_mx4(torch.randn(n, k, device=DEV))
+    x = torch.randn(9, k, device=DEV, dtype=torch.bfloat16)
+    want = mx_ops.linear_mx4(x, codes, scales)
+    for m in (1, 2, 7, 8):
+        assert torch.equal(mx_ops.linear_mx4(x[:m], codes, scales), want[:m])
+        for ld, first in ((k + 8, 0), (k + 8, 8), (k + 3, 0), (k + 8, 1), (2 * k, 0)):
+            wide = torch.full((m, ld + first), float("nan"), device=DEV, dtype=torch.bfloat16)
+            view = wide[:, first:first + k]
+            view.copy_(x[:m])
+            assert torch.equal(mx_ops.linear_mx4(view, codes, scales), want[:m]), (m, ld, first)
+    xc, xs, _ = mx_ops.add_rmsnorm_mx8(x, None, torch.ones(k, device=DEV))
+    want = mx_ops.linear_mx4(xc, codes, scales, x_scales=xs)
+    for m in (1, 2, 7, 8):
+        assert torch.equal(mx_ops.linear_mx4(xc[:m], codes, scales, x_scales=xs[:m]), want[:m])
+    assert torch.equal(want, mx_ops.linear_mx4(mx_ops.dequantize_mx8(xc, xs), codes, scales))
