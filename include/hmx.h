@@ -680,7 +680,8 @@ int hmx_mx_dequantize(const void* codes, const void* scales, int64_t n, int64_t 
 
 /* out (M, N) = x (M, K) * W^T for an mx4 table W (N, K).  x_kind 0: fp32 rows of stride ldx (elements), all 24 bits of a
  * value take part; 1: bfloat16; 2: mx8 codes (ldx = dp) with x_scales (M, dp / 32).  Bits of x below 2^-133 are left out
- * (mx8: rounded).  Sums in fp32; out contiguous, fp32 or bfloat16 (out_bf16 = 1). */
+ * (mx8: rounded).  Sums in fp32; out contiguous, fp32 or bfloat16 (out_bf16 = 1).  The workspace is 16-byte
+ * aligned. */
 size_t hmx_linear_mx4_workspace_bytes(int x_kind, int64_t M, int64_t K);
 int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, int x_kind, int64_t M, const void* codes, const void* scales,
                    int64_t N, int64_t K, int out_bf16, void* out, void* workspace, size_t workspace_bytes, void* stream);
@@ -696,8 +697,9 @@ int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, int x_kind,
  * Infinite maxima share the mass alone.  A row without candidates gives id -1 and probability 0.
  * u (B, draws) in [0, 1), fp64 where u_f64 = 1, else fp32; NaN and negative numbers count as 0, 1 and above as just
  * below 1.  temperature, top_k, top_p, min_p (B) or NULL: then the numbers behind them hold for every row.  Sums are
- * integers of a fixed unit per row (at most 2^-51 of the largest weight where the row's mass is below 2^11), so results
- * do not depend on the order of any addition.  V < 2^31, B < 2^22. */
+ * integers of a fixed unit per row (2^-51 of the largest weight, or more where a bound on the row's mass, at most 6 V,
+ * would not fit 62 bits of them), so results do not depend on the order of any addition.  V < 2^31, B < 2^22; the workspace
+ * is 16-byte aligned. */
 size_t hmx_sample_logits_workspace_bytes(int64_t B, int64_t V);
 int hmx_sample_logits(const void* logits, int64_t ld, int64_t B, int64_t V, int bf16, const void* u, int u_f64, int64_t draws,
                       const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,

@@ -70,7 +70,7 @@ def test_sample_entry():
         assert L.hmx_sample_logits(*{**good, **bad}.values()) == EINVAL, bad
     nbytes = L.hmx_sample_logits_workspace_bytes(4, 1 << 20)
     assert nbytes > 0 and L.hmx_sample_logits_workspace_bytes(4, 64) == 0
-    for bad in (dict(ws=P, ws_bytes=nbytes - 1), dict(ws=None, ws_bytes=nbytes)):
+    for bad in (dict(ws=P, ws_bytes=nbytes - 1), dict(ws=None, ws_bytes=nbytes), dict(ws=P + 8, ws_bytes=nbytes)):
         assert L.hmx_sample_logits(*{**good, "V": 1 << 20, "ld": 1 << 20, **bad}.values()) == -2
     assert L.hmx_sample_logits(*{**good, "B": 0, "logits": None}.values()) == 0
     assert L.hmx_sample_logits(*{**good, "draws": 0}.values()) == 0
