@@ -187,6 +187,9 @@ __device__ __forceinline__ Row settings(const SampleArgs& a, int64_t b) {
     Row r;
     r.k = a.top_k ? a.top_k[b] : a.k;
     if (!(t > 0.0) || t > 3e38) t = 1.0, r.k = 1;
+    // two fp32 scores lie 2^-149 apart at least: from here down all but the ones equal to the maximum weigh nothing, and
+    // 128 / (T ln 2) stays finite (times 0, for the maximum itself, infinity would be NaN)
+    t = fmax(t, 1e-60);
     if (r.k < 0 || r.k >= a.V) r.k = 0;
     r.p = p < 1.0 ? p : 1.0;
     r.inv_t = 1.0 / t;

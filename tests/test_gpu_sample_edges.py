@@ -1,0 +1,30 @@
+"""ops.sample_logits at the ends of what it accepts, against the definition in 64 bits (tests/test_gpu_sample.py: check, with
+its tolerances).  Row lengths reach each way that a row is worked on: whole in a list, by one block, cut over many blocks."""
+import sys
+
+import pytest
+import torch
+
+from generative_recommenders_amd import ops
+from test_gpu_sample import DEV, check, rows
+
+pytestmark = pytest.mark.gpu
+
+LENGTHS = [1500, 3000, 65537, 140001]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", LENGTHS)
+def test_smallest_temperatures(V, dtype):
+    """Down to the least positive double: the scores equal to the maximum share the draws, whatever else is set."""
+    logits, u = rows(3, V, 8, dtype, seed=V)
+    logits[1, ::V // 7] = logits[1].max()                 # 8 of them (or one less)
+    logits[2] = 0.0                                       # the smallest differences there are
+    logits[2, ::V // 5] = 1e-45 if dtype == torch.float32 else 1e-40
+    for t in (1e-50, 1e-300, sys.float_info.min, 1e-310, 5e-324):
+        for setting in (dict(), dict(k=3), dict(k=30), dict(p=0.7303), dict(k=2501, p=0.7303), dict(mp=0.5)):
+            ids, probs = check(logits, u, t=t, **setting)
+            assert bool((ids >= 0).all()) and bool((ids < V).all())
+            assert int((logits[0] == logits[0].max()).sum()) > 1 or bool((probs[0] == 1).all())
+            assert bool((logits.gather(1, ids) == logits.max(1, keepdim=True).values).all())
+    assert int(check(logits, u, t=5e-324)[0][1].unique().numel()) > 1
