@@ -213,6 +213,12 @@ __device__ __forceinline__ void set_scale(Row& r, float lmax, float most) {
     r.scale = min(51, 62 - ex);
     r.cut = -128.0 * (double)(r.scale + 2);
 }
+// exp((l - top) / T) in fp32, for bounds of a row's mass, with `by` = rough_by(r).  Halves, since finite scores may lie further
+// apart than the largest number; an infinite top leaves the others some weight where T is near it too: more is no harm.
+__device__ __forceinline__ float rough_by(const Row& r) { return fminf((float)(2.8853900817779268 * r.inv_t), kMaxFloat); }      // 2 / ln 2
+__device__ __forceinline__ float rough_weight(float l, float top, float by) {
+    return l == top ? 1.f : __builtin_amdgcn_exp2f(fmaxf(0.5f * l - 0.5f * top, -kMaxFloat) * by);
+}
 __device__ __forceinline__ void set_bins(Row& r, float range) {
     r.bin_scale = fminf((float)((double)kBins * r.inv_t) / range, kMaxFloat);
 }
@@ -937,14 +943,11 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
     st.need = 0;
     if (!candidate(top)) return;
     st.mode = kTiles;
-    const float by = (float)(1.4426950408889634 * r.inv_t);
+    const float by = rough_by(r);
     float mass = 0.f;
 #pragma unroll
-    for (int q = 0; q < kPerValue; ++q) mass += c[q] ? (float)c[q] * (l[q] == top ? 1.f : __builtin_amdgcn_exp2f((l[q] - top) * by)) : 0.f;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        const float x = entry_value(sh.list[i]);
-        mass += x == top ? 1.f : __builtin_amdgcn_exp2f((x - top) * by);
-    }
+    for (int q = 0; q < kPerValue; ++q) mass += c[q] ? (float)c[q] * rough_weight(l[q], top, by) : 0.f;
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) mass += rough_weight(entry_value(sh.list[i]), top, by);
     mass = block_sum(mass, sh);
     set_scale(r, top, fminf(mass * 1.01f + 1.f, (float)a.V));
     if (r.k == 0 && !(r.p < 1.0)) return;
@@ -1094,8 +1097,7 @@ __device__ __forceinline__ void row_by_bins(const SampleArgs& a, int64_t b, bool
         }
     }
     // the maxima of the threads bound the mass from below and, as often as a thread has elements, from above
-    const float by = (float)(1.4426950408889634 * r.inv_t);
-    const float least = 0.99f * block_sum(own == top ? 1.f : candidate(own) ? __builtin_amdgcn_exp2f((own - top) * by) : 0.f, sh);
+    const float least = 0.99f * block_sum(candidate(own) ? rough_weight(own, top, rough_by(r)) : 0.f, sh);
     set_scale(r, top, 1.03f * least * 4.f * (float)((a.V + 4 * kThreads - 1) / (4 * kThreads)));
     st.klo = 1, st.khi = 0;
     st.ties = 1;
@@ -1305,11 +1307,11 @@ __global__ __launch_bounds__(kThreads) void split_plan_kernel(SampleArgs a, RowS
             st.klo = key_by_maxima(r, groups, sh);
             st.mode = st.klo ? kGather : kAlone;
         } else if (r.k == 0) {
-            const float by = (float)(1.4426950408889634 * r.inv_t);
+            const float by = rough_by(r);
             float least = 0.f;
             for (int g = threadIdx.x; g < groups; g += kThreads) {
                 const float m = sh.group[g];
-                least += m == top ? 1.f : candidate(m) ? __builtin_amdgcn_exp2f((m - top) * by) : 0.f;
+                least += candidate(m) ? rough_weight(m, top, by) : 0.f;
             }
             least = 0.99f * block_sum(least, sh);
             const uint32_t tiles = (a.V + a.tile - 1) / a.tile, per = (tiles + groups / 64 - 1) / (groups / 64);

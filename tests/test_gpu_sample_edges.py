@@ -28,3 +28,17 @@ def test_smallest_temperatures(V, dtype):
             assert int((logits[0] == logits[0].max()).sum()) > 1 or bool((probs[0] == 1).all())
             assert bool((logits.gather(1, ids) == logits.max(1, keepdim=True).values).all())
     assert int(check(logits, u, t=5e-324)[0][1].unique().numel()) > 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", LENGTHS)
+def test_scores_further_apart_than_the_largest_number(V, dtype):
+    """All but one score 6.6e38 below it: at a temperature of 2.9e38 each of them weighs a tenth, and their mass counts."""
+    logits, u = rows(3, V, 8, dtype, seed=V + 2)
+    logits = (logits * 1e33 - 3.3e38).to(dtype)
+    logits[0, V // 3] = 3.3e38
+    logits[1, ::V // 7] = 3.3e38
+    logits[2, V - 1] = float("inf")
+    for t in (2.9e38, 1e38, 1e37):
+        for setting in (dict(), dict(k=30), dict(p=0.7303), dict(k=2501, p=0.7303), dict(mp=0.05)):
+            check(logits, u, t=t, **setting)
