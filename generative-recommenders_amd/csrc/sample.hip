@@ -186,10 +186,11 @@ __device__ __forceinline__ Row settings(const SampleArgs& a, int64_t b) {
     const double p = a.top_p ? (double)a.top_p[b] : a.p, mp = a.min_p ? (double)a.min_p[b] : a.mp;
     Row r;
     r.k = a.top_k ? a.top_k[b] : a.k;
-    if (!(t > 0.0) || t > 3e38) t = 1.0, r.k = 1;
-    // two fp32 scores lie 2^-149 apart at least: from here down all but the ones equal to the maximum weigh nothing, and
-    // 128 / (T ln 2) stays finite (times 0, for the maximum itself, infinity would be NaN)
-    t = fmax(t, 1e-60);
+    if (!(t > 0.0) || t == __builtin_inf()) t = 1.0, r.k = 1;
+    // two fp32 scores lie 2^-149 apart at least and 2^129 at most: below 1e-60 all but the ones equal to the maximum weigh
+    // nothing, above 1e60 all finite ones weigh the same to the last bit.  Within, 128 / (T ln 2) is finite (times 0, for the
+    // maximum itself, infinity would be NaN) and an infinite maximum's 1e300 still leaves the others nothing.
+    t = fmin(fmax(t, 1e-60), 1e60);
     if (r.k < 0 || r.k >= a.V) r.k = 0;
     r.p = p < 1.0 ? p : 1.0;
     r.inv_t = 1.0 / t;

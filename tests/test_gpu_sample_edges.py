@@ -42,3 +42,22 @@ def test_scores_further_apart_than_the_largest_number(V, dtype):
     for t in (2.9e38, 1e38, 1e37):
         for setting in (dict(), dict(k=30), dict(p=0.7303), dict(k=2501, p=0.7303), dict(mp=0.05)):
             check(logits, u, t=t, **setting)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", LENGTHS)
+def test_largest_temperatures(V, dtype):
+    """Every finite one is a temperature: all scores weigh the same, also where a row has float32's largest as its own."""
+    logits, u = rows(5, V, 8, dtype, seed=V + 3)
+    logits[1] = (logits[1] * 1e38).nan_to_num(0.0, 3e38, -3e38)
+    logits[2, V // 2] = float("inf")
+    logits[3, ::3] = float("-inf")
+    for t in (3.2e38, 1e39, 1e45, 1e59, 1e61, 1e300, sys.float_info.max):
+        for setting in (dict(), dict(k=30), dict(p=0.7303), dict(k=2501, p=0.7303), dict(mp=0.01)):
+            check(logits, u, t=t, **setting)
+    own = torch.tensor([3.1e38, 3.4028234e38, 1.0, 1e-45, float("inf")], device=DEV)
+    for setting in (dict(), dict(k=30), dict(p=0.7303)):
+        ids, probs = ops.sample_logits(logits, u, own, setting.get("k", 0), setting.get("p", 1.0))
+        want = check(logits, u, torch.where(torch.isfinite(own), own, torch.zeros_like(own)), **setting)
+        assert torch.equal(ids, want[0]) and torch.equal(probs, want[1])
+    assert int(ops.sample_logits(logits, u, own)[0][0].unique().numel()) > 4
