@@ -948,8 +948,13 @@ __device__ __forceinline__ void border_by_values(const SampleArgs& a, State& st,
     float mass = 0.f;
 #pragma unroll
     for (int q = 0; q < kPerValue; ++q) mass += c[q] ? (float)c[q] * rough_weight(l[q], top, by) : 0.f;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) mass += rough_weight(entry_value(sh.list[i]), top, by);
     mass = block_sum(mass, sh);
+    if (n) {                                                         // in the list's order, which changes: integers
+        u64 listed[1] = {0};
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) listed[0] += (u64)(rough_weight(entry_value(sh.list[i]), top, by) * 0x1p40f);
+        block_sums(listed, sh);
+        mass += (float)listed[0] * 0x1p-40f;
+    }
     set_scale(r, top, fminf(mass * 1.01f + 1.f, (float)a.V));
     if (r.k == 0 && !(r.p < 1.0)) return;
     // in descending order: the list above the counters' range, the positive values, the list between, the negative, the rest

@@ -61,3 +61,24 @@ def test_largest_temperatures(V, dtype):
         want = check(logits, u, torch.where(torch.isfinite(own), own, torch.zeros_like(own)), **setting)
         assert torch.equal(ids, want[0]) and torch.equal(probs, want[1])
     assert int(ops.sample_logits(logits, u, own)[0][0].unique().numel()) > 4
+
+
+@pytest.mark.parametrize("V", [6000, 80001])
+def test_the_same_scores_elsewhere_in_the_row(V):
+    """bfloat16 scores without a counter (below 2^-22, from 1024 on) are listed in the order that atomics give: rows that hold
+    the same scores in the same order, between other gaps, draw the same ones with the same probabilities."""
+    n, B = 3000, 8
+    g = torch.Generator(device=DEV).manual_seed(V)
+    scores = torch.cat([1024 + 8 * torch.randint(0, 3, (n // 2,), generator=g, device=DEV),
+                        1016 - 4 * torch.randint(0, 3, (n - n // 2,), generator=g, device=DEV)])
+    scores = scores[torch.randperm(n, generator=g, device=DEV)].bfloat16()
+    logits = torch.full((B, V), float("-inf"), dtype=torch.bfloat16, device=DEV)
+    at = torch.stack([torch.randperm(V, generator=g, device=DEV)[:n].sort().values for _ in range(B)])
+    logits.scatter_(1, at, scores.expand(B, n))
+    u = torch.rand(1, 500, generator=g, device=DEV, dtype=torch.float64).expand(B, 500)
+    for setting in (dict(t=7.0), dict(t=7.0, p=0.9), dict(t=7.0, k=2000), dict(t=30.0, k=2000, p=0.8, mp=0.1)):
+        ids, probs = ops.sample_logits(logits, u, setting["t"], setting.get("k", 0), setting.get("p", 1.0), setting.get("mp", 0.0))
+        rank = torch.searchsorted(at, ids)
+        assert torch.equal(at.gather(1, rank), ids)
+        assert torch.equal(rank, rank[:1].expand_as(rank)) and torch.equal(probs, probs[:1].expand_as(probs))
+        check(logits[:2], u[:2], **setting)
