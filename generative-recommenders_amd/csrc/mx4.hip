@@ -174,7 +174,9 @@ struct XTerms {
 };
 
 // v = h + m + l exactly: each term is the next 8 bits of the significand (cut, not rounded: no carry, and the largest finite
-// value stays finite).  An infinity or a NaN stays in the first term alone.
+// value stays finite).  An infinity or a NaN stays in the first term alone.  The others may be zero where v is not, and zero
+// times an infinite value of W (scale bytes 253 and 254) is NaN: what they would add to the first term's infinity, which has
+// their sign, is left out (add_term, finite).
 __device__ __forceinline__ XTerms<3> cut3(const float (&v)[8]) {
     uint32_t u[3][8];
 #pragma unroll
@@ -196,6 +198,19 @@ __device__ __forceinline__ XTerms<3> cut3(const float (&v)[8]) {
         t.p[q] = __builtin_bit_cast(bf16x8, w);
     }
     return t;
+}
+
+// The sum of the products with the first term, and that with a later one: NaN where that met an infinity (or where the first's is).
+__device__ __forceinline__ float add_term(float first, float later) { return later == later ? first + later : first; }
+// W for the later terms of an accumulator that the first term shares: the largest number in place of an infinity.
+__device__ __forceinline__ bf16x8 finite(bf16x8 v) {
+    u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & 0x7fffu) == 0x7f80u) w[i] -= 1u;
+        if ((w[i] & 0x7fff0000u) == 0x7f800000u) w[i] -= 0x10000u;
+    }
+    return __builtin_bit_cast(bf16x8, w);
 }
 
 // x[m, k .. k + 7] as exact bf16 terms; columns past K and rows past M read as zero.
@@ -331,9 +346,9 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
             const float s = block_ok ? scale_value(sc[t]) : 1.f;
             // rows that share an MFMA must not meet each other's infinities (6 * 2^126 and up) and NaN: zero times those
             // is NaN, so then W is masked to one row group at a time as well
-            const bool odd = R > 1 && __any(block_ok && sc[t] >= 253);
+            const bool odd = (R > 1 || PL > 1) && __any(block_ok && sc[t] >= 253);
             if constexpr (REP) {
-                if (odd) {
+                if (R > 1 && odd) {
                     f32x4 kept = {0.f, 0.f, 0.f, 0.f};
                     for (int g = 0; g < R; ++g) {
                         f32x4 one = {0.f, 0.f, 0.f, 0.f};
@@ -357,10 +372,11 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
                 } else {
 #pragma unroll
                     for (int g = 0; g < R; ++g) {
-                        const bf16x8 wg = odd ? zero_if(h != g, wv) : wv;
+                        const bf16x8 wg = R > 1 && odd ? zero_if(h != g, wv) : wv;
+                        const bf16x8 wl = PL > 1 && odd ? finite(wg) : wg;
 #pragma unroll
                         for (int q = 0; q < PL; ++q)
-                            acc[t * R + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(zero_if(R > 1 && h != g, xr[i][q]), wg,
+                            acc[t * R + g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(zero_if(R > 1 && h != g, xr[i][q]), q ? wl : wg,
                                                                                      acc[t * R + g], 0, 0, 0);
                     }
                 }
@@ -378,7 +394,7 @@ __global__ __launch_bounds__(256) void linear_short_kernel(LinearArgs a) {
             const int64_t n = tile * 64 + lane;                         // load t, row group of lane group j, table row c
             if (n < a.N) {
                 if constexpr (PL == 3) {
-                    store_out(out + n, (v[0] + v[1]) + v[2]);
+                    store_out(out + n, add_term(add_term(v[0], v[1]), v[2]));
                 } else {
 #pragma unroll
                     for (int m = 0; m < 4; ++m)
@@ -565,11 +581,11 @@ __global__ __launch_bounds__(64 * W) void linear_long_kernel(LinearArgs a, const
         const int col = e & 15, q = (e >> 4) % ROWS, rm = (e >> 4) / ROWS;
         float v = 0.f;
 #pragma unroll
-        for (int p = 0; p < TERMS; ++p) {
+        for (int p = 0; p < TERMS; ++p) {                            // the first term's sum, then the others'
             const int row = TERMS * q + p;
             float sum = 0.f;
             for (int k = 0; k < KW; ++k) sum += red[group * KW + k][rm * 4 + (row & 3)][(row >> 2) * 16 + col];
-            v += sum;
+            v = p ? add_term(v, sum) : sum;
         }
         const int m = ((int)blockIdx.y * MT + rm % MT) * ROWS + q;
         const int64_t n = n0 + 16 * (rm / MT) + col;

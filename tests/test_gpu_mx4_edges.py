@@ -1,0 +1,52 @@
+"""mx_ops.linear_mx4 at the ends of its range: table values that are infinite as float32 and bfloat16 (4 and 6 times 2^126, 2 to
+6 times 2^127), beside ordinary rows, whose tolerance is that of tests/test_gpu_mx4.py."""
+import pytest
+import torch
+
+from generative_recommenders_amd import mx_ops
+from test_gpu_mx4 import DEV, check_linear, operands
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "mx8"])
+@pytest.mark.parametrize("k", [32, 60, 64, 128, 300, 1000])
+@pytest.mark.parametrize("m", [1, 2, 6, 9, 20])
+def test_linear_infinite_table_values(m, k, kind):
+    """A value of x that is not zero times an infinity is one, of the product's sign, however few bits of x are set; two of
+    opposite signs make NaN.  (A zero of x times an infinity is NaN, so x holds none.)"""
+    n = 200
+    x, xs, x64, w64, codes, scales = operands(m, n, k, kind, seed=k + m)
+    ones = torch.ones_like(x64)
+    ones[:, 1::2] = -3.0
+    if m > 1 and kind != "mx8":                          # all bits of fp32 in one row, a few in the others
+        x64 = torch.cat([x64[:1], ones[1:]])
+        x64 = torch.where(x64 == 0, ones, x64)
+        x = x64.to(x.dtype)
+    elif kind == "mx8":
+        x, xs, _ = mx_ops.add_rmsnorm_mx8(ones.float(), None, torch.ones(k, device=DEV))
+        x64 = mx_ops.dequantize_mx8(x, xs, k, torch.float32).double()
+    else:
+        x64 = ones
+        x = ones.to(x.dtype)
+    codes, scales = codes.clone(), scales.clone()
+    rows = {}
+    for row, (byte, code) in enumerate([(253, 6), (253, 7), (254, 4), (254, 7), (253, 14), (254, 15)]):
+        for col in (0, k // 2, k - 1):
+            at = 30 * row + col % 7 + (col > 0) + (col == k - 1)     # distinct rows, neighbours of ordinary ones
+            codes[at] = 0
+            codes[at, col // 2] = code << (4 * (col & 1))
+            scales[at, col // 32] = byte
+            rows[at] = -1.0 if code > 7 else 1.0, col
+    both = 199                                           # infinities of both signs (of one sign where x's differ)
+    codes[both] = 0
+    codes[both, 0] = 0x76
+    scales[both, 0] = 254
+    out = mx_ops.linear_mx4(x, codes, scales, xs)
+    for at, (sign, col) in rows.items():
+        want = sign * torch.sign(x64[:, col]) * float("inf")
+        assert torch.equal(out[:, at].double(), want), (at, col)
+    same = torch.sign(x64[:, 0]) == torch.sign(x64[:, 1])
+    assert torch.equal(out[:, both].isnan(), ~same) and bool(out[same, both].isinf().all())
+    keep = torch.tensor([i for i in range(n) if i not in rows and i != both], device=DEV)
+    check_linear(out[:, keep], x64, w64[keep])
