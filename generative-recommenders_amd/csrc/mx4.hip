@@ -714,7 +714,12 @@ extern "C" int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, 
     if (M < 0 || N < 0 || K < 1 || K > (1 << 26) || ldx < 0 || x_kind < 0 || x_kind > 2) return HMX_EINVAL;
     if (M == 0 || N == 0) return HMX_OK;
     if (!x || !codes || !scales || !out || !aligned(codes, 16) || (x_kind == kXMx8) != (x_scales != nullptr)) return HMX_EINVAL;
-    if (M > 65535 * 16 || hmx_ceil_div(N, 32) > (1 << 22)) return HMX_EINVAL;        // the grid's limits
+    // the grid's limits: 65535 blocks in y, 2^32 threads in x
+    if (M > 65535 * 16 || hmx_ceil_div(N, 32) > (1 << 22)) return HMX_EINVAL;
+    if (K > 128) {
+        const int64_t tiles = operand_tiles(x_kind, M), chunks = 2 * hmx_ceil_div(K, 256);
+        if (hmx_ceil_div(tiles, 2) > 65535 || tiles * chunks * (x_kind == kXMx8 ? 128 : 256) > (int64_t)UINT32_MAX - 256) return HMX_EINVAL;
+    }
     if (x_kind == kXMx8 && (K % 32 || !aligned(x, 16))) return HMX_EINVAL;
     const LinearArgs a = {x, ldx, (const uint8_t*)x_scales, (int)M, (const u32x4*)codes, (const uint8_t*)scales, N, (int)K,
                           (int)hmx_ceil_div(K, 32), out};

@@ -681,7 +681,8 @@ int hmx_mx_dequantize(const void* codes, const void* scales, int64_t n, int64_t 
 /* out (M, N) = x (M, K) * W^T for an mx4 table W (N, K).  x_kind 0: fp32 rows of stride ldx (elements), all 24 bits of a
  * value take part; 1: bfloat16; 2: mx8 codes (ldx = dp) with x_scales (M, dp / 32).  Bits of x below 2^-133 are left out
  * (mx8: rounded); table values from 2^128 on count as infinite, and zero times these is NaN.  Sums in fp32; out contiguous,
- * fp32 or bfloat16 (out_bf16 = 1).  The workspace is 16-byte aligned. */
+ * fp32 or bfloat16 (out_bf16 = 1).  The workspace is 16-byte aligned.  M is at most 1,048,560, N 2^27; of rows longer than 128
+ * at most 655,350 where x is fp32, and the tiles of 16 rows (fp32: 5) times K, rounded up to 256, stay below 2^31 (mx8: 2^32). */
 size_t hmx_linear_mx4_workspace_bytes(int x_kind, int64_t M, int64_t K);
 int hmx_linear_mx4(const void* x, int64_t ldx, const void* x_scales, int x_kind, int64_t M, const void* codes, const void* scales,
                    int64_t N, int64_t K, int out_bf16, void* out, void* workspace, size_t workspace_bytes, void* stream);
