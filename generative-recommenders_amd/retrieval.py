@@ -341,7 +341,7 @@ class SampledRetriever:
     values, fp32 sums), draws follow ops.sample_logits (temperature, top_k, top_p, min_p; numbers or one per state).  Against
     search() of ShardedRetriever, which returns the best k, this explores: probs is what each item was drawn with.  The
     table takes 17 / 32 of a byte per value (a quarter of its bf16 copy); scores of a chunk of states are held in memory,
-    `score_bytes` of them at most."""
+    `score_bytes` of them at most (one state's at least)."""
 
     def __init__(self, table, id_offset=0, score_bytes=1 << 30):
         self.id_offset = int(id_offset)
@@ -395,6 +395,7 @@ class SampledRetriever:
                 sc.scatter_reduce_(1, torch.where(inside, row, items - 1), torch.where(inside, float("-inf"), keep), "amin")
             t, k, p, mp = (s[part] if isinstance(s, torch.Tensor) else s for s in settings)
             ids[part], probs[part] = ops.sample_logits(sc, u[part], t, k, p, mp)
+            del sc                                    # before the next chunk's are made
         if self.id_offset:
             ids = torch.where(ids >= 0, ids + self.id_offset, ids)
         return ids, probs
