@@ -377,10 +377,20 @@ class SampledRetriever:
         """u (n,) or (n, draws) in [0, 1): the random numbers.  exclude (n, any) int64: item ids never drawn for a state
         (entries outside the table are ignored).  A state without a drawable item gets id -1."""
         from . import hmx, ops
+        if states.dim() != 2 or states.shape[1] != self.dim:
+            raise hmx.HmxError(f"SampledRetriever: states are (n, {self.dim}), got {tuple(states.shape)}")
         n, items = states.shape[0], self.codes.shape[0]
         if u.shape[:1] != (n,) or u.dim() > 2:
             raise hmx.HmxError(f"SampledRetriever: u is ({n},) or ({n}, draws), got {tuple(u.shape)}")
         settings = (temperature, top_k, top_p, min_p)
+        # here and not in the chunks, which would take the first rows of more than there are states
+        if residual is not None and residual.shape != states.shape:
+            raise hmx.HmxError(f"SampledRetriever: residual {tuple(residual.shape)} does not match states {tuple(states.shape)}")
+        if exclude is not None and (exclude.dim() != 2 or exclude.shape[0] != n or exclude.dtype != torch.int64):
+            raise hmx.HmxError(f"SampledRetriever: exclude is int64 ({n}, any), got {exclude.dtype} {tuple(exclude.shape)}")
+        for name, value in zip(("temperature", "top_k", "top_p", "min_p"), settings):
+            if isinstance(value, torch.Tensor) and value.shape != (n,):
+                raise hmx.HmxError(f"SampledRetriever: {name} is a number or a ({n},) tensor, got {tuple(value.shape)}")
         step = max(1, self.score_bytes // (4 * max(1, items)))
         ids = torch.empty(u.shape, dtype=torch.int64, device=u.device)
         probs = torch.empty(u.shape, dtype=torch.float32, device=u.device)
