@@ -352,11 +352,13 @@ class SampledRetriever:
     def refresh(self, table):
         """Call after the table's weights changed: quantises it again, into the same memory where its shape is the same (a
         captured sample() then reads the new weights)."""
-        from . import mx_ops
+        from . import hmx, mx_ops
+        if table.dim() != 2:
+            raise hmx.HmxError(f"SampledRetriever: the table is a matrix, got {tuple(table.shape)}")
         same = self.codes is not None and self.codes.device == table.device and \
             (self.codes.shape[0], self.dim) == tuple(table.shape)
-        self.dim = table.shape[1]
         self.codes, self.scales = mx_ops.quantize_mx4(table.detach(), (self.codes, self.scales) if same else None)
+        self.dim = table.shape[1]                     # a table that is refused leaves the old one whole
 
     def scores(self, states, norm_scale=None, residual=None, eps=1e-6):
         """(n, d) states -> (n, items) fp32 scores.  norm_scale (d,): the states are first added to `residual` (where given)

@@ -41,3 +41,18 @@ def test_operands_of_another_number_of_states_are_refused(score_bytes):
             rt.sample(states, u[:states.shape[0]])
     got = rt.sample(h, u, temperature=seven[:5], top_k=seven[:5].int(), exclude=ex[:5, :0])
     assert torch.equal(got[0], rt.sample(h, u, top_k=1)[0])
+
+
+def test_a_refused_table_leaves_the_old_one():
+    table, h, res, scale, u = setup(n=5, items=5003, seed=6)
+    rt = SampledRetriever(table)
+    want = rt.sample(h, u, top_p=0.9)
+    for bad in (table[:, :60].half(), table[:, :40].cpu(), table[:, :0], table[0]):
+        with pytest.raises(hmx.HmxError):
+            rt.refresh(bad)
+        got = rt.sample(h, u, top_p=0.9)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        with pytest.raises(hmx.HmxError):
+            rt.sample(h[:, :60], u)
+    rt.refresh(table[:, :60])
+    assert rt.sample(h[:, :60], u)[0].shape == u.shape
