@@ -614,6 +614,6 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     nbytes = hmx.lib().hmx_sample_logits_workspace_bytes(b, v)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _launch("hmx_sample_logits", device, rows.data_ptr(), rows.stride(0), b, v, int(logits.dtype == torch.bfloat16), u.data_ptr(),
-            int(u.dtype == torch.float64), draws, hmx.ptr(t), hmx.ptr(k), hmx.ptr(p), hmx.ptr(mp), float(t_all), int(k_all),
+            int(u.dtype == torch.float64), draws, hmx.ptr(t), hmx.ptr(k), hmx.ptr(p), hmx.ptr(mp), float(t_all), min(int(k_all), v),
             float(p_all), float(mp_all), ids.data_ptr(), probs.data_ptr(), hmx.ptr(ws), nbytes)
     return ids, probs

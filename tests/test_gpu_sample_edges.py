@@ -82,3 +82,12 @@ def test_the_same_scores_elsewhere_in_the_row(V):
         assert torch.equal(at.gather(1, rank), ids)
         assert torch.equal(rank, rank[:1].expand_as(rank)) and torch.equal(probs, probs[:1].expand_as(probs))
         check(logits[:2], u[:2], **setting)
+
+
+@pytest.mark.parametrize("V", [1500, 70001])
+def test_top_k_past_64_bits(V):
+    logits, u = rows(2, V, 50, seed=V)
+    want = ops.sample_logits(logits, u)
+    for k in (V, V + 1, 2 ** 63 - 1, 2 ** 63, 2 ** 64 + 5, 10 ** 30):
+        got = ops.sample_logits(logits, u, top_k=k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
