@@ -370,7 +370,7 @@ int dispatch_fwd(const FwdArgs& a, hipStream_t st) {
     if (vec) {
         const int nvec = width / V;
 #define CALL(LPR, NV)                                                              \
-    if constexpr (NV <= 8) launch_fwd<T, V, LPR, NV, MX8>(a, st)
+    if constexpr (LPR * NV <= kMaxD / V) launch_fwd<T, V, LPR, NV, MX8>(a, st)
         HMX_NORM_WIDTHS(CALL)
 #undef CALL
     } else if constexpr (MX8) {
@@ -414,7 +414,7 @@ int dispatch_bwd(const BwdArgs& a, hipStream_t st) {
     if (vec) {
         const int nvec = a.d / V;
 #define CALL(LPR, NV)                                                              \
-    if constexpr (NV <= 8) launch_bwd<T, V, LPR, NV>(a, st)
+    if constexpr (LPR * NV <= kMaxD / V) launch_bwd<T, V, LPR, NV>(a, st)
         HMX_NORM_WIDTHS(CALL)
 #undef CALL
     } else {
