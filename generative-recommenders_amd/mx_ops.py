@@ -24,7 +24,7 @@ def padded(d):
 
 def add_rmsnorm_mx8(x, residual, scale, eps=1e-6):
     """enc_ops.add_rmsnorm with y in mx8 -> (codes float8_e4m3fn (..., dp), scales uint8 (..., dp / 32), s); residual
-    None: s is x.  The codes come from the float32 y; no gradient."""
+    None: s is x.  Statistics and y are float64, and y is rounded once, to its code; no gradient."""
     device, x2, r2, bf16 = _norm_operands("add_rmsnorm_mx8", x, residual, scale, eps)
     T, d = x2.shape
     dp = padded(d)

@@ -1,0 +1,70 @@
+"""mx_ops.add_rmsnorm_mx8: codes and scales are the ones of the exact values.  Both sides take their statistics in 64 bits and
+differ by some 2^-52 in each of a few steps; values (and largest values of a block) within 1e-13 of a border between two codes
+(or scales) are left out, at most one in a thousand."""
+import pytest
+import torch
+
+from generative_recommenders_amd import mx_ops
+from test_gpu_add_rmsnorm import DEV, EPS, SHAPES, formula, least_exponent, make
+
+pytestmark = pytest.mark.gpu
+NEAR = 1e-13
+
+
+def e4m3(a):
+    """Magnitudes (at most 448) rounded to nearest even, and how near they are to a border, relative."""
+    exp = (torch.frexp(a)[1] - 1).clamp_min(-6)
+    step = torch.exp2((exp - 3).double())
+    q = a / step
+    return torch.round(q) * step, ((q - torch.floor(q) - 0.5).abs() / q.clamp_min(0.5))
+
+
+def check_exact(s, w, eps, codes, scales):
+    d, dp = s.shape[-1], mx_ops.padded(s.shape[-1])
+    y = torch.zeros(s.shape[0], dp, dtype=torch.float64, device=DEV)
+    y[:, :d] = formula(s, w, eps=eps)
+    amax = y.view(s.shape[0], -1, 32).abs().amax(2)
+    e = least_exponent(amax)
+    near = least_exponent(amax * (1 - NEAR)) != least_exponent(amax * (1 + NEAR))
+    assert torch.equal((scales.double() - 127)[~near], e[~near])
+    unit = torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+    want, gap = e4m3(y.abs() / unit)
+    left_out = (gap < NEAR) | near.repeat_interleave(32, 1)
+    assert float(left_out.double().mean()) <= 1e-3
+    got = codes.double()
+    assert torch.equal(got[~left_out].abs(), want[~left_out])
+    assert torch.equal(torch.signbit(got)[:, :d], torch.signbit(y)[:, :d])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,d", SHAPES)
+def test_mx8_codes_are_those_of_the_exact_values(T, d, dtype):
+    x, r, w, _, _ = make(T, d, dtype, 19)
+    codes, scales, s = mx_ops.add_rmsnorm_mx8(x, r, w, EPS)
+    check_exact(s, w, EPS, codes, scales)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 65])
+def test_mx8_beside_a_tie(d, dtype):
+    """y a 2^-30 of itself beside the middle of two codes, nearer than fp32 can tell: below it (by eps) everywhere, above it (by
+    one smaller element of the row) in fp32.  Rounded to fp32 first, it would be a tie, and go to the even code."""
+    ties = torch.tensor([1.0625, 1.1875, 1.3125, 1.4375, 1.5625, 1.6875, 1.8125, 1.9375], dtype=torch.float64)
+    w = torch.ones(d, dtype=torch.float64)
+    w[0] = w[32] = 256.0                                  # a scale of 1
+    w[1:9], w[9:17], w[40:48] = ties, -64 * ties, ties / 64
+    below = torch.ones(3, d, dtype=dtype, device=DEV)
+    codes, scales, s = mx_ops.add_rmsnorm_mx8(below, None, w.float().to(DEV), 2.0 ** -29)
+    assert bool((scales[:, :2] == 127).all())
+    floor = torch.floor(ties * 8) / 8
+    got = codes.double().cpu()
+    assert torch.equal(got[:, 1:9], floor.expand(3, 8)) and torch.equal(got[:, 9:17], -64 * floor.expand(3, 8))
+    assert torch.equal(got[:, 40:48], floor.expand(3, 8) / 64)
+    check_exact(s, w.float().to(DEV), 2.0 ** -29, codes, scales)
+    if dtype == torch.float32:
+        above = below.clone()
+        above[:, 20] = 1 - 2.0 ** -24
+        codes, scales, s = mx_ops.add_rmsnorm_mx8(above, None, w.float().to(DEV), 0.0)
+        got = codes.double().cpu()
+        assert torch.equal(got[:, 1:9], floor.expand(3, 8) + 0.125) and torch.equal(got[:, 40:48], (floor.expand(3, 8) + 0.125) / 64)
+        check_exact(s, w.float().to(DEV), 0.0, codes, scales)
