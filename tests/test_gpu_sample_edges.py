@@ -91,3 +91,46 @@ def test_top_k_past_64_bits(V):
     for k in (V, V + 1, 2 ** 63 - 1, 2 ** 63, 2 ** 64 + 5, 10 ** 30):
         got = ops.sample_logits(logits, u, top_k=k)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+
+
+def kinds(B):
+    """Settings of B rows, neighbours of different kinds: greedy, a small top_k, one above 2000, top_p, min_p, all of them, and
+    none; with those, a row worked on by maxima, by bins, by narrowing and by tiles stand side by side."""
+    t = torch.tensor([0.0, 1.0, 0.7, 1.0, 1.3, 1.0, 1.0, float("inf")], device=DEV).repeat(-(-B // 8))[:B]
+    k = torch.tensor([0, 20, 2500, 0, 0, 300, 0, 5], dtype=torch.int32, device=DEV).repeat(-(-B // 8))[:B]
+    p = torch.tensor([1.0, 1.0, 0.93, 0.87, 1.0, 0.8, 1.0, 1.0], device=DEV).repeat(-(-B // 8))[:B]
+    mp = torch.tensor([0.0, 0.0, 0.001, 0.0, 0.03, 0.01, 0.0, 0.0], device=DEV).repeat(-(-B // 8))[:B]
+    return t, k, p, mp
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,V", [(10, 9001), (10, 70001), (10, 300001), (64, 65536), (3, 1_000_003)])
+def test_rows_of_every_kind_beside_each_other(B, V, dtype):
+    """Each row's draws are those of its own settings, also where one launch cuts rows of different kinds over many blocks."""
+    logits, u = rows(B, V, 7, dtype, seed=V + B)
+    if B >= 10:
+        logits[9] = float("-inf")                         # nothing to draw
+        logits[4, ::2] = float("nan")
+        logits[6] = 0.25                                  # one score for the whole row
+        logits[3, 1::2] = logits[3, 0]                    # a border among equal scores
+    t, k, p, mp = kinds(B)
+    got = ops.sample_logits(logits, u, t, k, p, mp)
+    plain_t = torch.where(torch.isfinite(t), t, torch.zeros_like(t))
+    some = torch.arange(min(B, 10), device=DEV)
+    want = check(logits[some], u[some], plain_t[some], k[some], p[some], mp[some])
+    for a, b in zip(got, want):
+        assert torch.equal(a[some], b)
+    for i in range(B):                                    # alone, with numbers for settings
+        one = ops.sample_logits(logits[i], u[i], plain_t[i].item(), int(k[i]), p[i].item(), mp[i].item())
+        assert torch.equal(one[0], got[0][i])
+        # by its length and the number of rows a row is worked on in ways whose scales differ: a rounding of a weight, 2^-24 of probs
+        assert bool(((one[1] - got[1][i]).abs() <= 2.0 ** -23 * got[1][i]).all())
+
+
+def test_probabilities_are_the_shares():
+    logits, u = rows(3, 700, 2000, seed=12)
+    ids, probs = ops.sample_logits(logits, u, top_k=40)
+    kept = torch.topk(logits, 40).values[:, -1:]
+    w = torch.where(logits >= kept, torch.exp(logits.double() - logits.double().max(1, keepdim=True).values), torch.zeros_like(logits).double())
+    want = (w / w.sum(1, keepdim=True)).gather(1, ids)
+    assert bool(((probs.double() - want).abs() <= (2.0 ** -24 + 1e-9) * want).all())
