@@ -1,7 +1,8 @@
 // Tables and layers in 4 bits: blocks of 32 values of a row share a power-of-two scale (e8m0 byte), values are e2m1.
 //
 // quantize / dequantize: one pass, bound by HBM.  A lane owns 8 columns, four lanes a block of 32.  4,000,001 x 64: fp32 to
-// 4 bits 230 us (5.05 TB/s), to bf16 131 us (4.95 TB/s); a copy of 1 GiB reaches 5.1 TB/s.
+// 4 bits 230 us (5.05 TB/s), to bf16 131 us (4.95 TB/s); a copy of 1 GiB reaches 5.1 TB/s.  Widths that are no multiple of 8 are
+// read and written element by element: x 60 fp32 to 4 bits 245 us (4.5 TB/s), back 577 (1.9; bf16 237 and 310).
 //
 // linear: out[m, n] = sum_k x[m, k] W[n, k] for few rows of x, bound by the bytes of W (and by out where it is wide).  A
 // lane loads one block of W (16 bytes, 32 codes); v_cvt_scalef32_pk_bf16_fp4 turns two codes and the scale into two bf16
@@ -287,6 +288,8 @@ __device__ __forceinline__ void transpose_groups(float (&v)[4]) {
 
 // K <= 128 (scores of a table of embeddings): x stays in registers, waves walk the table 64 rows at a time.
 // Bound by HBM: 1 row x 4,000,001 x 64 27.8 us (152 MB, 5.5 TB/s), 16 rows x 1,000,003 x 60 22.2 us (98 MB, 64 of them written).
+// Several fp32 rows (three terms each, one MFMA a term and row group) are bound by those and by their registers: 4 rows x
+// 4,000,001 x 64 78 us (2.6 TB/s), 16 rows 108 (3.6; bf16 101), 67 rows, five passes over the table, 465 (bf16 450).
 // With one or two blocks a row (R = 4 or 2), the lane groups of one load hold R groups of 16 rows, so that a load still is
 // 1 KB of consecutive codes; the MFMA would add the groups up, so x is zero in the lane groups of the other row groups:
 //   REP (planes * M <= 4): rows 4 j + i of the x operand hold term / row i for lane group j's own row group, so that lane

@@ -9,6 +9,10 @@
 // (its operands partly from cache); 16,384 x 4096 bf16 forward 92 (5.8 TB/s), backward 112 + 6 (4.8 TB/s, 17 MB of partials
 // included: 4 blocks a compute unit keep them few); 8191 x 1000 fp32 into 8 bits 22.9 (4.7 TB/s); 1024 x 64: 3.3 and 5.7,
 // 1 x 4096 into 8 bits 4.3: the launch.
+// Rows whose width is no multiple of the vector go column by column: 8191 x 1001 bf16 forward 23.5, into 8 bits 35.7 (1000 columns:
+// 12.5, 16.1).  Wide rows spill registers: backward past 16,384 columns (102 fp32, 103 bf16; 1024 x 32,768 278 and 254 us, 1.9 and
+// 1.1 TB/s; forward, which does not, 111 and 60), and the single-column 8-bit form past 8192 (713 fp32, 2696 bf16: 1024 x 20,001
+// 882 and 2560 us, against 104 and 62 at 20,000 columns).
 #include "hmx_common.h"
 
 #include <algorithm>
@@ -21,7 +25,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxD = 32768;
-constexpr int64_t kFewRows = 2048;      // up to this many the backward pass is one launch
+// Up to this many rows the backward pass is one launch, whose blocks for dscale read s and dy again.  One launch / two, us, fp32:
+// 256 x 64 4.5 / 5.1, 1024 x 64 4.8 / 5.8, 2048 x 64 6.7 / 5.6, 4096 x 64 16.3 / 5.8; 1024 x 1024 9.6 / 12.3, 2048 x 1024 15.2 / 14.1;
+// 256 x 8192 13.5 / 12.2, 1024 x 8192 47.9 / 41.6, 2048 x 8192 89 / 65.  The border is where a step of few kernels gains the most: there
+// the host's time counts, and a launch and a buffer less with it.
+constexpr int64_t kFewRows = 2048;
 constexpr int kBwdBlocks = 1024;      // rows of weight-gradient partials at most (4 blocks per CU)
 
 template <typename T>

@@ -23,8 +23,8 @@
 //   ordered 32-bit key, three looks at most, until a range is one key.
 // One block does a row on its own; few long rows are cut into segments for the looks at all elements, with one block a row
 // between them.
-// Measured, us: 256 x 131,072 bf16 47 in one launch: the count of values 9.5, the border from 8192 counters 8, the tiles 14, the
-// draws 6 (67 MB once at 5.1 TB/s: 13); 4 x 4,000,001 fp32, top_k 1000 and 16 draws 44: maxima 12, plan 6, gather 13, list and
+// Measured, us: 256 x 131,072 bf16 44.6 in one launch: start and cleared counters 2.9, the count of values 12, the border from 8192
+// counters 10, the tiles 14.7, the draws 5.1 (67 MB once at 5.1 TB/s: 13); 4 x 4,000,001 fp32, top_k 1000 and 16 draws 44: maxima 12, plan 6, gather 13, list and
 // draws 13; 1 x 50,000 fp32, top_k 50: 12.
 #include "hmx_common.h"
 
@@ -1198,6 +1198,10 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
 }
 
 // ------------------------------------------------------------------------------- many blocks, one row
+// row_by_bins on one block is the slow way, six to eight reads of the row: fp32 with a top_k that the groups' maxima do not lead to a
+// list (above 819 on one block, 51 for each block of a cut row, or 2000; or, the k-th of them more than 32 T below the maximum), lists
+// that overflow, bfloat16 with more than 4096 scores that have no counter.  1 x 4,000,001 fp32 top_k 1000 29 us, 3000 1715, with
+// top_p 3494; 256 x 131,072 fp32 top_k 800 53, 1000 126; 1 x 50,000 top_k 50 13, at T = 0.05 39; bf16 256 x 131,072 half of it zeros 112.
 // Between the kernels a row's state lies in the workspace.  The looks run on gridDim.x segments of whole tiles a row, the
 // steps between them on one block a row.
 struct RowSpace {
@@ -1345,6 +1349,8 @@ struct SharedLook {
     u64 mass;
     uint32_t n_list, base;
 };
+// Two blocks a compute unit leave 64 registers: the fp32 form spills 45.  With / without that bound: 4 x 4,000,001 top_p 0.9 131 /
+// 131 us, no border 47 / 45, 64 x 131,072 33.4 / 33.2, with top_p 66.5 / 60.4.
 template <typename T>
 __global__ __launch_bounds__(kThreads, 8) void split_look_kernel(SampleArgs a, RowSpace* ws) {
     __shared__ SharedLook sh;
@@ -1441,7 +1447,7 @@ __global__ __launch_bounds__(kThreads) void split_border_kernel(SampleArgs a, Ro
 //   64 x   131,072         18 /  22         63 /  64         40 / 30          41 / 38
 //  128 x   131,072         27 /  36         72 /  93         47 / 45          41 / 45
 // Where every row leads to a list by a small top_k, one block looks at it but twice: 1 x 262,144 24 / 17, 32 x 262,144 25 / 21,
-// 64 x 500,000 52 / 53.
+// 64 x 500,000 52 / 53.  Rows of a larger batch are not cut, however long: 4,000,001 fp32, top_p 0.9, 64 rows 929, 67 rows 2264.
 int splits(int64_t B, int64_t V) {
     const int64_t c = std::min<int64_t>(std::min<int64_t>(512 / B, V / 4096), kMaxSplit);
     return V >= 1 << 16 && c >= 8 ? (int)c : 1;

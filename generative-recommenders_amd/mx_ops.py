@@ -106,8 +106,9 @@ def linear_mx4(x, codes, scales, x_scales=None, out_dtype=torch.float32):
     """out (..., N) = x (..., K) times the transposed mx4 table (codes (N, dp / 2), scales (N, dp / 32)), dp = padded(K).
 
     x is float32 (all 24 bits take part), bfloat16, or mx8 codes (..., dp) with x_scales (..., dp / 32); bits of x below
-    2^-133 are left out.  Sums are float32, out is float32 or bfloat16; no gradient.  Made for few rows of x: the scores of a batch of users over an item table, a
-    layer for single tokens.  More rows re-read the table once per 32 (layers) or 16 (K <= 128)."""
+    2^-133 are left out, and table values from 2^128 on count as infinite.  Sums are float32, out is float32 or bfloat16;
+    no gradient.  Made for few rows of x: the scores of a batch of users over an item table, a layer for single tokens.  More
+    rows re-read the table once per 16 (K <= 128), or 32 (10 where x is float32)."""
     device, n, blocks, codes, scales = _checked("linear_mx4", codes, scales, torch.uint8, BLOCK // 2)
     if scales.dim() != 2:
         raise hmx.HmxError(f"linear_mx4: the table is a matrix, got codes {tuple(codes.shape)}")
