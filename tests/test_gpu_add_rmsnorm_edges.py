@@ -1,10 +1,10 @@
 """mx_ops.add_rmsnorm_mx8: codes and scales are the ones of the exact values.  Both sides take their statistics in 64 bits and
 differ by some 2^-52 in each of a few steps; values (and largest values of a block) within 1e-13 of a border between two codes
-(or scales) are left out, at most one in a thousand."""
+(or scales) are left out, at most one in a thousand.  enc_ops.add_rmsnorm: a training step captured into a graph."""
 import pytest
 import torch
 
-from generative_recommenders_amd import mx_ops
+from generative_recommenders_amd import enc_ops, mx_ops
 from test_gpu_add_rmsnorm import DEV, EPS, SHAPES, formula, least_exponent, make
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,38 @@ def test_mx8_beside_a_tie(d, dtype):
         got = codes.double().cpu()
         assert torch.equal(got[:, 1:9], floor.expand(3, 8) + 0.125) and torch.equal(got[:, 40:48], (floor.expand(3, 8) + 0.125) / 64)
         check_exact(s, w.float().to(DEV), 0.0, codes, scales)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,d", [(300, 128), (5000, 64), (2049, 1001)])
+def test_gradients_in_a_graph_and_on_a_stream(T, d, dtype):
+    """Forward and backward of both row counts' ways (one launch, and partial sums in a workspace), replayed with eager steps of
+    other tensors and of the same sizes between: no replay meets another's memory."""
+    x, r, w, dy, ds = make(T, d, dtype, 23)
+
+    def step(x, r, w):
+        leaves = [t.detach().requires_grad_() for t in (x, r, w)]
+        y, s = enc_ops.add_rmsnorm(*leaves)
+        return (y, s) + torch.autograd.grad((y, s), leaves, (dy, ds))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = step(x, r, w)
+    torch.cuda.current_stream().wait_stream(side)
+    want = step(x, r, w)
+    assert all(torch.equal(a, b) for a, b in zip(on_side, want))
+    graphs = []
+    for _ in range(2):
+        xs = x.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(xs, r, w)
+        graphs.append((graph, xs, out))
+    for k in range(4):
+        graph, xs, out = graphs[k % 2]
+        xs.copy_(x * (1 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(x * (1 + k), r, w)
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), k
