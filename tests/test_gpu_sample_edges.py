@@ -134,3 +134,26 @@ def test_probabilities_are_the_shares():
     w = torch.where(logits >= kept, torch.exp(logits.double() - logits.double().max(1, keepdim=True).values), torch.zeros_like(logits).double())
     want = (w / w.sum(1, keepdim=True)).gather(1, ids)
     assert bool(((probs.double() - want).abs() <= (2.0 ** -24 + 1e-9) * want).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_longest_rows(dtype):
+    """2^31 - 1 scores, the most there may be: equal ones (each index its share, the lowest kept), and three among -infinity."""
+    V = 2 ** 31 - 1
+    logits = torch.ones(1, V, dtype=dtype, device=DEV)
+    at = torch.tensor([0, 1, 12345, 2 ** 30 + 5, 2 ** 31 - 2 - 4096, V - 1], device=DEV)
+    u = ((at.double() + 0.5) / V).view(1, -1)
+    ids, probs = ops.sample_logits(logits, u)
+    assert torch.equal(ids[0], at) and bool(((probs.double() * V - 1).abs() <= 2.0 ** -23).all())
+    if dtype == torch.bfloat16:                           # (equal fp32 scores are counted in one place: seconds at this length)
+        half = u / 2                                          # top_p 0.5 keeps the first 2^30 (of 2^31 - 1 equal shares)
+        ids, probs = ops.sample_logits(logits, half, top_p=0.5)
+        assert torch.equal(ids[0], (half[0] * 2 ** 30).floor().long()) and bool(((probs.double() * 2 ** 30 - 1).abs() <= 2.0 ** -23).all())
+        ids, probs = ops.sample_logits(logits, u, top_k=5)
+        assert torch.equal(ids[0], (u[0] * 5).floor().long()) and bool(((probs.double() * 5 - 1).abs() <= 2.0 ** -23).all())
+    logits.fill_(float("-inf"))
+    three = torch.tensor([7, V - 2 ** 20, V - 1], device=DEV)
+    logits[0, three] = 2.0
+    for setting in (dict(), dict(top_k=100), dict(top_p=0.9), dict(temperature=0.1, min_p=0.5)):
+        ids, probs = ops.sample_logits(logits, u, **setting)
+        assert torch.equal(ids[0], three[(u[0] * 3).floor().long()]) and bool(((probs.double() * 3 - 1).abs() <= 2.0 ** -23).all()), setting
