@@ -103,3 +103,34 @@ def test_gradients_in_a_graph_and_on_a_stream(T, d, dtype):
         torch.cuda.synchronize()
         want = step(x * (1 + k), r, w)
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,d", [((1 << 24) + (1 << 20) + 3, 8), ((1 << 31) // 32768 + 9, 32768), (70001, 30721)])
+def test_rows_past_the_grid_and_past_32_bits(T, d, dtype):
+    """More rows than one round of blocks takes, and offsets past 2^31 elements: rows at the ends and in the middle are the ones
+    that a call with these rows alone gives."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, d, generator=g, device=DEV, dtype=dtype)
+    r = torch.randn(1, d, generator=g, device=DEV, dtype=dtype).expand(T, d)
+    w = 1 + 0.2 * torch.randn(d, generator=g, device=DEV)
+    parts = [slice(0, 3), slice(T // 2, T // 2 + 3), slice(T - 7, T)]
+
+    def same(got, f):
+        for p in parts:
+            for a, b in zip(got, f(p)):
+                assert torch.equal(a[p].view(torch.uint8), b.view(torch.uint8))
+
+    same(enc_ops.add_rmsnorm(x, r, w), lambda p: enc_ops.add_rmsnorm(x[p], r[p], w))
+    same(mx_ops.add_rmsnorm_mx8(x, r, w), lambda p: mx_ops.add_rmsnorm_mx8(x[p], r[p], w))
+    leaf = x.requires_grad_()
+    y, s = enc_ops.add_rmsnorm(leaf, r, w)
+    del s
+    dx = torch.autograd.grad(y, leaf, y.detach())[0]      # dy = y
+    del y
+
+    def alone(p):
+        small = x.detach()[p].clone().requires_grad_()
+        y, _ = enc_ops.add_rmsnorm(small, r[p], w)
+        return torch.autograd.grad(y, small, y.detach())
+    same([dx], alone)

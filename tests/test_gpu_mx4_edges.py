@@ -50,3 +50,17 @@ def test_linear_infinite_table_values(m, k, kind):
     assert torch.equal(out[:, both].isnan(), ~same) and bool(out[same, both].isinf().all())
     keep = torch.tensor([i for i in range(n) if i not in rows and i != both], device=DEV)
     check_linear(out[:, keep], x64, w64[keep])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d", [(70_000_003, 32), (1_100_003, 2001)])
+def test_tables_past_the_grid_and_past_32_bits(n, d, dtype):
+    """More octets than one round of blocks takes (the first), more than 2^31 values: parts of the table are what they give alone."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    table = torch.randn(n, d, generator=g, device=DEV, dtype=dtype)
+    codes, scales = mx_ops.quantize_mx4(table)
+    back = mx_ops.dequantize_mx4(codes, scales, d, dtype)
+    for at in (0, n // 2, n - 1000):
+        c, s = mx_ops.quantize_mx4(table[at:at + 1000].clone())
+        assert torch.equal(codes[at:at + 1000], c) and torch.equal(scales[at:at + 1000], s)
+        assert torch.equal(back[at:at + 1000], mx_ops.dequantize_mx4(c, s, d, dtype))
