@@ -24,8 +24,8 @@
 // One block does a row on its own; few long rows are cut into segments for the looks at all elements, with one block a row
 // between them.
 // Measured, us: 256 x 131,072 bf16 44.6 in one launch: start and cleared counters 2.9, the count of values 12, the border from 8192
-// counters 10, the tiles 14.7, the draws 5.1 (67 MB once at 5.1 TB/s: 13); 4 x 4,000,001 fp32, top_k 1000 and 16 draws 44: maxima 12, plan 6, gather 13, list and
-// draws 13; 1 x 50,000 fp32, top_k 50: 12.
+// counters 10, the tiles 14.7, the draws 5.1 (67 MB once at 5.1 TB/s: 13); 4 x 4,000,001 fp32, top_k 1000 and 16 draws 44: maxima
+// 12, plan 6, gather 13, list and draws 13; 1 x 50,000 fp32, top_k 50: 12.
 #include "hmx_common.h"
 
 #include <algorithm>

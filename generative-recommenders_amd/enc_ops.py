@@ -173,7 +173,8 @@ def add_rmsnorm(x, residual, scale, eps=1e-6):
     """s = x + residual (rounded to their type), y = s * (mean(s^2) + eps)^(-1/2) * scale -> (y, s).
 
     x and residual (..., d) are float32 or bfloat16 with any strides, 1 <= d <= 32768, scale (d,) is float32; sums are
-    float32 (a row whose squares add up to 2^128 or more gives zeros, below 2^-126 they lose bits).  residual None: the norm of x, -> (y, x).  Gradients flow from y and from s to x, residual and scale."""
+    float32 (a row whose squares add up to 2^128 or more gives zeros, below 2^-126 they lose bits).  residual
+    None: the norm of x, -> (y, x).  Gradients flow from y and from s to x, residual and scale."""
     if residual is None:
         return _AddRMSNorm.apply(x, None, scale, eps), x
     return _AddRMSNorm.apply(x, residual, scale, eps)

@@ -651,7 +651,8 @@ int hmx_attn_bwd(const float* q, const float* kv, const float* drop, const float
 /* s = x + residual (rounded to the tensors' type), y = s * (mean(s^2) + eps)^(-1/2) * scale over the last dimension.
  * x, residual, s, y are fp32 (bf16 = 0) or bfloat16 (bf16 = 1), scale and rstd fp32; sums in fp32 (a row whose squares
  * add up to 2^128 or more gives zeros, below 2^-126 they lose bits).  x and residual are (T, d) with row strides ldx / ldr
- * in elements (0: one row for all), s, y contiguous.  residual NULL: the norm of x (s may then be NULL).  rstd (T) or NULL receives the factor for the backward pass.  1 <= d <= 32768, eps >= 0. */
+ * in elements (0: one row for all), s, y contiguous.  residual NULL: the norm of x (s may then be NULL).  rstd (T) or NULL
+ * receives the factor for the backward pass.  1 <= d <= 32768, eps >= 0. */
 int hmx_add_rmsnorm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* scale, int64_t T,
                         int64_t d, double eps, int bf16, void* s, void* y, float* rstd, void* stream);
 
